@@ -18,6 +18,7 @@ INCLUDE = PKG.parent / "include"
 _lib = None
 
 u32, i32, u64, f32 = ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_float
+f64 = ctypes.c_double
 vp = ctypes.c_void_p
 szt = ctypes.c_size_t
 
@@ -71,6 +72,13 @@ DAV2CUDA = {
     "dav2cuda_conv_transpose_half": (ctypes.c_int, [vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, vp, u64, vp]),
     "dav2cuda_attention_head64": (ctypes.c_int, [vp, vp, u32, u32, u32, vp, u64, vp]),
     "dav2cuda_attention_head64_workspace_size": (u64, [u32, u32, u32]),
+    "dav2cuda_rope_frequencies": (ctypes.c_int, [vp, vp, u32, u32, f64, u32, f64, f64]),
+    "dav2cuda_qk_norm_rope": (ctypes.c_int, [vp] * 10 + [u32] * 6 + [u64] * 4 + [u32, f32, u32, f32, u32, u32, vp]),
+    "dav2cuda_kv_cache_append_s8": (ctypes.c_int, [vp] * 9 + [u32] * 7 + [u64] * 2 + [u32, vp]),
+    "dav2cuda_attention_cache_s8_workspace_size": (u64, [u32] * 6),
+    "dav2cuda_attention_cache_s8": (ctypes.c_int, [vp] * 9 + [u32] * 9 + [u64] * 2 + [f32, u32, u32, u32, vp, u64, vp]),
+    "dav2cuda_cross_attention_16_workspace_size": (u64, [u32] * 6),
+    "dav2cuda_cross_attention_16": (ctypes.c_int, [vp] * 5 + [u32] * 6 + [u64] * 8 + [f32, u32, u32, vp, u64, vp]),
     "dav2cuda_linear_half_workspace_size": (u64, [u32, u32, u32]),
     "dav2cuda_linear_half": (ctypes.c_int, [vp, vp, vp, vp, u32, u32, u32, u32, u32, vp, u64, vp]),
     "dav2cuda_conv2d_half_workspace_size": (u64, [u32, u32, u32, u32, u32, u32, u32]),

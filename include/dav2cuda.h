@@ -49,7 +49,8 @@ typedef enum dav2cuda_status {
 DAV2CUDA_API const char* dav2cuda_last_error(void);
 DAV2CUDA_API const char* dav2cuda_build_info(void);
 /* Reads and clears the device error word that kernels set instead of
- * trapping (1 = a pipeline wait timed out). Synchronizes the device. */
+ * trapping (1 = a pipeline wait timed out, 3 = a length, offset or page in a
+ * device array was out of range). Synchronizes the device. */
 DAV2CUDA_API int dav2cuda_device_error(void);
 /* Number of kernels this library launched since the last reset. */
 DAV2CUDA_API uint64_t dav2cuda_launch_count(int reset);
@@ -399,6 +400,127 @@ DAV2CUDA_API int dav2cuda_attention_head64(float* output, const float* qkv, uint
                                            uint64_t workspace_bytes, void* stream);
 DAV2CUDA_API uint64_t dav2cuda_attention_head64_workspace_size(uint32_t batch, uint32_t tokens,
                                                                uint32_t heads);
+
+/* ------------------------------------- transformer operators (extensions) */
+
+/* What transformers beyond the reference's encoder need next to the entries
+ * above: norms and rotary positions of queries and keys, a paged 8-bit cache of
+ * keys and values with the attention that reads it, and attention to another
+ * set of tokens. No counterpart in the reference.
+ *
+ * "precision" numbers a type: 0 f32, 1 bf16, 2 f16. Strides are in elements of
+ * the tensor's type, from one token to the next (the heads of a token lie one
+ * after another), so that a part of a packed q|k|v row can be passed in place.
+ * Device arrays of lengths, offsets and pages are read by the kernels; a value
+ * out of range is never used as an address: the work that it belongs to is left
+ * out (a length is clamped) and the device error word becomes 3. */
+
+/* Rotary frequencies, computed on the host: frequency j of each axis =
+ * base^(-j / count), count = rotary_dim / 2 / axes, host_frequencies
+ * [rotary_dim / 2], axis after axis. scaling, for positions beyond a trained
+ * length: 0 none; 1 positions divided by factor; 2 the base raised so that the
+ * lowest frequency is divided by factor and the highest kept; 3 by bands:
+ * frequencies that make 32 turns or more over trained_length are kept, those that
+ * make one or less divided by factor, those between in linear proportion, and
+ * *host_rotary_scale = 0.1 ln(factor) + 1 (otherwise 1). factor >= 1. */
+DAV2CUDA_API int dav2cuda_rope_frequencies(float* host_frequencies, float* host_rotary_scale,
+                                           uint32_t rotary_dim, uint32_t axes, double base,
+                                           uint32_t scaling, double factor, double trained_length);
+
+/* Norm of each head of q and k and rotation by position, in one pass.
+ * q [tokens][q_heads][head_dim], k [tokens][k_heads][head_dim] (q_heads or
+ * k_heads may be 0). norm: 0 none; 1 x * rsqrt(mean(x^2) + epsilon) * weight +
+ * bias; 2 the same of x - mean(x); weight [head_dim] and bias [head_dim] f32,
+ * each may be NULL (1 and 0). Then, with a = positions[token][axis] *
+ * frequencies[pair] (positions NULL: the token's index; one axis), each pair
+ * (u, v) of the first rotary_dim values becomes rotary_scale * (u cos a - v sin a,
+ * v cos a + u sin a). layout: 0 pair i = values i and i + rotary_dim/2; 1 values
+ * 2i and 2i + 1; 2 halves within each axis's rotary_dim/axes values. Pairs are
+ * numbered axis after axis, rotary_dim/2/axes to each. head_dim even, up to
+ * 256. Output of the input's type, or of any type for f32 input. Outputs may be
+ * the inputs themselves (same type and stride). Sizes, strides and addresses
+ * that allow 16-byte accesses (head_dim and rotary_dim multiples of 16) are
+ * fastest. */
+DAV2CUDA_API int dav2cuda_qk_norm_rope(void* q_output, void* k_output, const void* q, const void* k,
+                                       const float* q_weight, const float* q_bias,
+                                       const float* k_weight, const float* k_bias,
+                                       const float* frequencies, const int32_t* positions,
+                                       uint32_t tokens, uint32_t q_heads, uint32_t k_heads,
+                                       uint32_t head_dim, uint32_t rotary_dim, uint32_t axes,
+                                       uint64_t q_output_stride, uint64_t k_output_stride,
+                                       uint64_t q_stride, uint64_t k_stride, uint32_t norm,
+                                       float epsilon, uint32_t layout, float rotary_scale,
+                                       uint32_t input_precision, uint32_t output_precision,
+                                       void* stream);
+
+/* Appends rows to a paged cache of int8 codes. codes [page_count][kv_heads]
+ * [page_tokens][head_dim] and scales [page_count][kv_heads], of K and of V;
+ * sequence s has token t in page page_table[s * table_stride + t / page_tokens]
+ * at t % page_tokens. Its new rows are rows token_begin[s] .. token_begin[s + 1]
+ * of k and v ([tokens][kv_heads][head_dim]), which follow the cached[s] tokens it
+ * holds. scale = max(absmax / 127, 1e-8) and code = rint(clamp(x / scale)) over
+ * each page and head, as dav2cuda_quantize_rows_s8 has them for rows; a page that
+ * holds tokens keeps its scale unless the new rows need a larger one, and its
+ * codes then become rint(code * (old scale / new scale)). Infinities take the
+ * codes +-127 and NaN the code 0; neither enters a scale. Places behind the last
+ * token stay as they were. page_tokens 16, 32, 64 or 128, head_dim a multiple of
+ * 16 up to 128. A page that receives rows may belong to one sequence only;
+ * sequences may share full pages. 16-byte aligned rows and codes. */
+DAV2CUDA_API int dav2cuda_kv_cache_append_s8(int8_t* k_codes, float* k_scales, int8_t* v_codes,
+                                             float* v_scales, const void* k, const void* v,
+                                             const int32_t* page_table, const int32_t* cached,
+                                             const int32_t* token_begin, uint32_t sequences,
+                                             uint32_t tokens, uint32_t kv_heads, uint32_t head_dim,
+                                             uint32_t page_count, uint32_t page_tokens,
+                                             uint32_t table_stride, uint64_t k_stride,
+                                             uint64_t v_stride, uint32_t precision, void* stream);
+
+/* Attention over that cache: softmax(scale * q . k) . v. Sequence s has the
+ * query rows query_begin[s] .. query_begin[s + 1] of q ([queries][q_heads]
+ * [head_dim], bf16 or f16) and lengths[s] <= max_length tokens in the cache, the
+ * new ones included. causal != 0: its queries are its last tokens, query i of n
+ * sees the first lengths[s] - n + i + 1 tokens. Query head h reads key head
+ * h / (q_heads / kv_heads). A query that sees nothing gives zeros; rows of no
+ * sequence stay as they were. Output f32 or of q's type. Products with f16
+ * operands (codes exactly, q scaled by a power of two, softmax weights rounded
+ * to f16) and f32 accumulation. workspace_size answers for the same numbers. */
+DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint32_t sequences, uint32_t queries,
+                                                                 uint32_t max_length, uint32_t q_heads,
+                                                                 uint32_t kv_heads, uint32_t head_dim);
+DAV2CUDA_API int dav2cuda_attention_cache_s8(void* output, const void* q, const int8_t* k_codes,
+                                             const float* k_scales, const int8_t* v_codes,
+                                             const float* v_scales, const int32_t* page_table,
+                                             const int32_t* lengths, const int32_t* query_begin,
+                                             uint32_t sequences, uint32_t queries, uint32_t max_length,
+                                             uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
+                                             uint32_t page_count, uint32_t page_tokens,
+                                             uint32_t table_stride, uint64_t q_stride,
+                                             uint64_t output_stride, float scale, uint32_t causal,
+                                             uint32_t precision, uint32_t output_precision,
+                                             void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Attention of q [batch][queries][q_heads][head_dim] to k and v [batch][keys]
+ * [kv_heads][head_dim], bf16 or f16: softmax(scale * q . k) . v over the first
+ * key_lengths[b] keys (key_lengths NULL: all). Keys behind that are not read
+ * into the result, whatever they hold; a batch entry without keys gives zeros.
+ * head_dim a multiple of 8 up to 128; 16-byte aligned rows; batch and token
+ * strides as given. Query head h reads key head h / (q_heads / kv_heads). Output
+ * f32 or of the operands' type. f32 accumulation, softmax weights rounded to the
+ * operands' type. workspace_size answers for the same numbers. */
+DAV2CUDA_API uint64_t dav2cuda_cross_attention_16_workspace_size(uint32_t batch, uint32_t queries,
+                                                                 uint32_t keys, uint32_t q_heads,
+                                                                 uint32_t kv_heads, uint32_t head_dim);
+DAV2CUDA_API int dav2cuda_cross_attention_16(void* output, const void* q, const void* k, const void* v,
+                                             const int32_t* key_lengths, uint32_t batch,
+                                             uint32_t queries, uint32_t keys, uint32_t q_heads,
+                                             uint32_t kv_heads, uint32_t head_dim,
+                                             uint64_t q_batch_stride, uint64_t q_stride,
+                                             uint64_t k_batch_stride, uint64_t k_stride,
+                                             uint64_t v_batch_stride, uint64_t v_stride,
+                                             uint64_t output_batch_stride, uint64_t output_stride,
+                                             float scale, uint32_t precision,
+                                             uint32_t output_precision, void* workspace,
+                                             uint64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------ fp32 family */
 
