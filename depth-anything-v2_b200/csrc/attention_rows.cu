@@ -33,11 +33,7 @@
 // at the end in shared memory, or (many rows) four row tiles and the same keys, which
 // they then find in L1. Where there are few row tiles, the keys of a tile are split
 // over several blocks whose (o, m, sum) go to the workspace, and a second kernel joins them.
-#include <algorithm>
-#include <cmath>
-
-#include "abi_check.h"
-#include "kernels.cuh"
+#include "attention_rows.cuh"
 
 namespace dav2cuda {
 namespace {
@@ -46,36 +42,6 @@ constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr uint32_t kChunk = 32;   // keys of one step of a warp
 constexpr float kRaise = 8.0f;    // m is raised when a score exceeds it by this
-
-struct RowsParams {
-    void* out;
-    const void* q;
-    const void* k;
-    const void* v;
-    const float* k_scales;
-    const float* v_scales;
-    const int32_t* page_table;
-    const int32_t* lengths;      // keys of each sequence (null: all)
-    const int32_t* query_begin;  // null: sequence s has rows [s * queries, (s + 1) * queries)
-    uint64_t q_batch, q_stride, k_batch, k_stride, v_batch, v_stride, out_batch, out_stride;
-    uint32_t sequences, queries, max_length, group, kv_heads, head_dim, pages, page_shift, table_stride;
-    uint32_t causal, row_warps, splits, q_bf16, out_kind;  // out_kind: 0 f32, 1 bf16, 2 f16
-    float scale_log2;
-    float* part_o;   // [query][head][split][head_dim]
-    float2* part_ml; // [query][head][split]
-    int* err;
-};
-
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t s) { return __byte_perm(a, b, s); }
-
-__device__ __forceinline__ uint32_t hsub2_1152(uint32_t x) {
-    uint32_t y;
-    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));
-    return y;
-}
-// Codes in bytes 0, 1 (2, 3) of x, offset by 128, as two f16 values.
-__device__ __forceinline__ uint32_t codes_lo(uint32_t x) { return hsub2_1152(prmt(x, 0x64646464u, 0x4140)); }
-__device__ __forceinline__ uint32_t codes_hi(uint32_t x) { return hsub2_1152(prmt(x, 0x64646464u, 0x4342)); }
 
 template <bool kBF16>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -94,34 +60,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-
-template <bool kBF16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (kBF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    } else {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-}
-
-__device__ __forceinline__ float2 unpack2(uint32_t x, bool bf16) {
-    if (bf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
-    return __half22float2(*reinterpret_cast<const __half2*>(&x));
-}
-
-__device__ __forceinline__ void store_out(const RowsParams& p, uint64_t at, const float* x, uint32_t n) {
-    if (p.out_kind == 0) {
-        float* o = static_cast<float*>(p.out) + at;
-        for (uint32_t i = 0; i < n; i += 2) *reinterpret_cast<float2*>(o + i) = make_float2(x[i], x[i + 1]);
-    } else {
-        uint16_t* o = static_cast<uint16_t*>(p.out) + at;
-        for (uint32_t i = 0; i < n; i += 2)
-            *reinterpret_cast<uint32_t*>(o + i) =
-                p.out_kind == 1 ? pack2<true>(x[i], x[i + 1]) : pack2<false>(x[i], x[i + 1]);
-    }
 }
 
 // One 16-key tile of codes or of 16-bit rows in registers.
@@ -231,54 +169,14 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     const uint32_t tile_rows = R * p.row_warps, key_warps = kWarps / p.row_warps;
     const uint32_t row_warp = warp / key_warps, key_warp = warp % key_warps;
 
-    // the sequence and the row tile of this block
+    RowTile where;
+    if (!find_row_tile(where, p, blockIdx.x, tile_rows)) return;
     Where w;
     w.kv_head = blockIdx.y;
-    uint32_t s = 0, q_begin, q_count, tile;
-    if (p.query_begin) {
-        for (uint32_t high = p.sequences; high - s > 1;) {
-            const uint32_t mid = (s + high) / 2;
-            if ((uint64_t)(uint32_t)p.query_begin[mid] * p.group / tile_rows + mid <= blockIdx.x) s = mid;
-            else high = mid;
-        }
-        const int32_t b = p.query_begin[s], e = p.query_begin[s + 1];
-        if (b < 0 || e < b || (uint32_t)e > p.queries) {
-            if (threadIdx.x == 0) atomicExch(p.err, 3);
-            return;
-        }
-        const uint64_t slot = (uint64_t)b * p.group / tile_rows + s;
-        if (blockIdx.x < slot) return;
-        q_begin = b, q_count = e - b;
-        tile = (uint32_t)(blockIdx.x - slot);
-    } else {
-        const uint32_t tiles = (p.queries * p.group + tile_rows - 1) / tile_rows;
-        s = blockIdx.x / tiles;
-        tile = blockIdx.x - s * tiles;
-        q_begin = 0, q_count = p.queries;
-    }
-    w.seq = s;
-    const uint32_t rows = q_count * p.group;
-    if ((uint64_t)tile * tile_rows >= rows) return;
-    int32_t length = p.lengths ? p.lengths[s] : (int32_t)p.max_length;
-    if (length < 0 || (uint32_t)length > p.max_length) {
-        if (threadIdx.x == 0) atomicExch(p.err, 3);
-        length = length < 0 ? 0 : (int32_t)p.max_length;
-    }
-    w.len = (uint32_t)length;
-    const uint32_t row0 = tile * tile_rows + row_warp * R;  // this warp's first row
-
-    auto reach_of = [&](uint32_t row) -> uint32_t {
-        if (row >= rows) return 0;
-        if (!p.causal) return w.len;
-        const int64_t r = (int64_t)w.len - q_count + row / p.group + 1;
-        return r > 0 ? (uint32_t)r : 0;
-    };
-    auto row_at = [&](uint32_t row, uint64_t batch, uint64_t stride) -> uint64_t {  // element of a live row
-        const uint32_t i = row / p.group;
-        const uint32_t head = w.kv_head * p.group + row - i * p.group;
-        const uint64_t token = (uint64_t)q_begin + i;
-        return (p.query_begin ? 0 : s * batch) + token * stride + (uint64_t)head * p.head_dim;
-    };
+    w.seq = where.seq;
+    w.len = keys_of(p, where.seq);
+    const uint32_t rows = where.rows;
+    const uint32_t row0 = where.tile * tile_rows + row_warp * R;  // this warp's first row
 
     // q as the products' B fragments, and the factors of its rows
     uint32_t qf[NT][kSteps][2];
@@ -287,7 +185,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t row = row0 + 8 * n + g;
-        const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row < rows ? row_at(row, p.q_batch, p.q_stride) : 0);
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row < rows ? row_at(p, where, w.kv_head, row, p.q_batch, p.q_stride) : 0);
         float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
@@ -323,7 +221,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             factor[n][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e)) * p.scale_log2;
-            reach[n][e] = reach_of(row0 + 8 * n + 2 * t + e);
+            reach[n][e] = reach_of(p, where, w.len, row0 + 8 * n + 2 * t + e);
             low = min(low, reach[n][e]);
             high = max(high, reach[n][e]);
         }
@@ -498,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     // merge the key warps of each row tile: a thread takes two dims of a row
     for (uint32_t i = threadIdx.x; i < R * p.row_warps * (D / 2); i += kThreads) {
         const uint32_t r = i / (D / 2), dim = 2 * (i - r * (D / 2));
-        const uint32_t rw = r / R, col = r - rw * R, row = tile * tile_rows + r;
+        const uint32_t rw = r / R, col = r - rw * R, row = where.tile * tile_rows + r;
         if (row >= rows || dim >= p.head_dim) continue;
         float top = -INFINITY;
         for (uint32_t k = 0; k < key_warps; ++k) top = fmaxf(top, s_m[rw * key_warps + k][col]);
@@ -514,12 +412,9 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         if (p.splits == 1) {
             const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
             x[0] *= inv, x[1] *= inv;
-            store_out(p, row_at(row, p.out_batch, p.out_stride) + dim, x, 2);
+            store_out(p, row_at(p, where, w.kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
         } else {
-            const uint32_t qi = row / p.group;
-            const uint64_t token = (p.query_begin ? 0ull : (uint64_t)s * p.queries) + q_begin + qi;
-            const uint64_t slot = (token * (p.kv_heads * p.group) + w.kv_head * p.group + row - qi * p.group) *
-                                      p.splits + blockIdx.z;
+            const uint64_t slot = part_at(p, where, w.kv_head, row, blockIdx.z);
             if (dim == 0) p.part_ml[slot] = make_float2(top, sum);
             if (sum > 0.0f) *reinterpret_cast<float2*>(p.part_o + slot * p.head_dim + dim) = make_float2(x[0], x[1]);
         }
@@ -562,190 +457,31 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const RowsPara
     if (dim < p.head_dim) store_out(p, (p.query_begin ? flat : at) + dim, x, 4);
 }
 
-struct Plan {
-    uint32_t row_tiles;  // 8-row tiles of a warp
-    uint32_t row_warps;
-    uint32_t splits;
-    uint64_t slots;
-};
-
-// Rows that share a key head decide the tile; the keys are split where the row
-// tiles alone would leave SMs idle, down to 256 keys to a block.
-Plan plan_rows(uint64_t sequences, uint64_t queries, bool ragged, uint32_t max_length, uint32_t group,
-               uint32_t kv_heads, uint32_t sms) {
-    Plan n;
-    const uint64_t each = ragged ? (queries + sequences - 1) / sequences : queries;
-    const uint64_t rows = each * group;
-    n.row_tiles = rows <= 8 ? 1 : 2;
-    n.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    const uint64_t tile = 8ull * n.row_tiles * n.row_warps;
-    n.slots = ragged ? queries * group / tile + sequences : sequences * ((rows + tile - 1) / tile);
-    const uint64_t live = std::max<uint64_t>(1, sequences * ((rows + tile - 1) / tile)) * kv_heads;
-    const uint64_t want = (3ull * sms + live - 1) / live;
-    const uint64_t most = std::max<uint64_t>(1, max_length / 256);
-    n.splits = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(want, most), 128);
-    return n;
-}
-
-uint64_t workspace_of(const Plan& n, uint64_t tokens, uint32_t heads, uint32_t head_dim) {
-    if (n.splits == 1) return 0;
-    return tokens * heads * n.splits * (head_dim * 4ull + 8) + 256;
-}
-
-template <int D, int NT, bool kS8, bool kBF16>
-void start(const RowsParams& p, const Plan& n, cudaStream_t st) {
-    attention_rows_kernel<D, NT, kS8, kBF16>
-        <<<dim3((uint32_t)n.slots, p.kv_heads, n.splits), kThreads, 0, st>>>(p);
-}
-
 template <bool kS8, bool kBF16>
-void start_for(const RowsParams& p, const Plan& n, cudaStream_t st) {
+void start_for(const RowsParams& p, uint32_t slots, uint32_t row_tiles, cudaStream_t st) {
+    const dim3 grid(slots, p.kv_heads, p.splits);
     if (p.head_dim <= 64) {
-        if (n.row_tiles == 1) start<64, 1, kS8, kBF16>(p, n, st);
-        else start<64, 2, kS8, kBF16>(p, n, st);
+        if (row_tiles == 1) attention_rows_kernel<64, 1, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
+        else attention_rows_kernel<64, 2, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
     } else {
-        if (n.row_tiles == 1) start<128, 1, kS8, kBF16>(p, n, st);
-        else start<128, 2, kS8, kBF16>(p, n, st);
+        if (row_tiles == 1) attention_rows_kernel<128, 1, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
+        else attention_rows_kernel<128, 2, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
     }
 }
 
-int run_rows(RowsParams& p, const Plan& n, bool s8, bool bf16, uint64_t tokens, void* workspace, cudaStream_t st) {
-    p.row_warps = n.row_warps, p.splits = n.splits;
-    if (n.splits > 1) {
-        const uint64_t slots = tokens * p.kv_heads * p.group * n.splits;
-        uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
-        p.part_o = reinterpret_cast<float*>(base);
-        p.part_ml = reinterpret_cast<float2*>(base + slots * p.head_dim * 4);
-    }
-    if (s8) start_for<true, false>(p, n, st);
-    else if (bf16) start_for<false, true>(p, n, st);
-    else start_for<false, false>(p, n, st);
-    if (int rc = check_launch("attention_rows")) return rc;
-    if (n.splits == 1) return DAV2CUDA_OK;
-    const uint64_t rows = tokens * p.kv_heads * p.group;
+}  // namespace
+
+int launch_attention_rows(const RowsParams& p, uint32_t slots, uint32_t row_tiles, bool s8, bool bf16,
+                          cudaStream_t st) {
+    if (s8) start_for<true, false>(p, slots, row_tiles, st);
+    else if (bf16) start_for<false, true>(p, slots, row_tiles, st);
+    else start_for<false, false>(p, slots, row_tiles, st);
+    return check_launch("attention_rows");
+}
+
+int launch_attention_join(const RowsParams& p, uint64_t rows, cudaStream_t st) {
     attention_join_kernel<<<(uint32_t)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(p);
     return check_launch("attention_join");
 }
 
-bool shape_ok(uint32_t q_heads, uint32_t kv_heads) {
-    return q_heads >= 1 && kv_heads >= 1 && kv_heads <= 65535 && q_heads % kv_heads == 0 && q_heads <= 65535;
-}
-
-}  // namespace
 }  // namespace dav2cuda
-
-using namespace dav2cuda;
-
-// The sizes are answered for 148 SMs, a B200's, so that they need no device.
-constexpr uint32_t kPlanSms = 148;
-
-extern "C" DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint32_t sequences, uint32_t queries,
-                                                                            uint32_t max_length, uint32_t q_heads,
-                                                                            uint32_t kv_heads, uint32_t head_dim) {
-    if (!sequences || !queries || !shape_ok(q_heads, kv_heads)) return 0;
-    const Plan n = plan_rows(sequences, queries, true, max_length, q_heads / kv_heads, kv_heads, kPlanSms);
-    return workspace_of(n, queries, q_heads, head_dim);
-}
-
-extern "C" DAV2CUDA_API int dav2cuda_attention_cache_s8(
-    void* output, const void* q, const int8_t* k_codes, const float* k_scales, const int8_t* v_codes,
-    const float* v_scales, const int32_t* page_table, const int32_t* lengths, const int32_t* query_begin,
-    uint32_t sequences, uint32_t queries, uint32_t max_length, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,
-    uint32_t page_count, uint32_t page_tokens, uint32_t table_stride, uint64_t q_stride, uint64_t output_stride,
-    float scale, uint32_t causal, uint32_t precision, uint32_t output_precision, void* workspace,
-    uint64_t workspace_bytes, void* stream) {
-    DAV2_REQUIRE(precision == 1 || precision == 2, "cache attention: queries must be bf16 or f16");
-    DAV2_REQUIRE(output_precision == 0 || output_precision == precision,
-                 "cache attention: output must be f32 or of the queries' type");
-    DAV2_REQUIRE(shape_ok(q_heads, kv_heads), "cache attention: q_heads must be a multiple of kv_heads");
-    DAV2_REQUIRE(head_dim >= 16 && head_dim <= 128 && head_dim % 16 == 0,
-                 "cache attention: head_dim must be a multiple of 16, 16 to 128");
-    DAV2_REQUIRE(page_tokens >= 16 && page_tokens <= 128 && (page_tokens & (page_tokens - 1)) == 0,
-                 "cache attention: page_tokens must be 16, 32, 64 or 128");
-    DAV2_REQUIRE(page_count >= 1 && page_count <= 0x7FFFFFFFu && table_stride >= 1 && max_length <= 0x7FFFFF00u &&
-                     (uint64_t)table_stride * page_tokens >= max_length,
-                 "cache attention: the page table does not hold max_length tokens");
-    DAV2_REQUIRE(std::isfinite(scale), "cache attention: invalid scale");
-    DAV2_REQUIRE((uint64_t)queries * (q_heads / kv_heads) <= 0x3FFFFFFFu && sequences <= 0x3FFFFFFFu,
-                 "cache attention: too many queries or sequences");
-    if (!queries || !sequences) return DAV2CUDA_OK;
-    const uint64_t row = (uint64_t)q_heads * head_dim;
-    DAV2_REQUIRE(queries == 1 || (q_stride >= row && output_stride >= row),
-                 "cache attention: a token stride is below the row of its heads");
-    DAV2_REQUIRE(!any_null(output, q, k_codes, k_scales, v_codes, v_scales, page_table, lengths, query_begin),
-                 "cache attention: null buffer");
-    DAV2_REQUIRE(aligned16(output) && aligned16(q) && aligned16(k_codes) && aligned16(v_codes) &&
-                     (queries == 1 || (q_stride % 8 == 0 && output_stride % 8 == 0)),
-                 "cache attention: rows must be 16-byte aligned");
-    RowsParams p{};
-    p.out = output, p.q = q, p.k = k_codes, p.v = v_codes, p.k_scales = k_scales, p.v_scales = v_scales;
-    p.page_table = page_table, p.lengths = lengths, p.query_begin = query_begin;
-    p.q_stride = q_stride, p.out_stride = output_stride;
-    p.sequences = sequences, p.queries = queries, p.max_length = max_length, p.group = q_heads / kv_heads;
-    p.kv_heads = kv_heads, p.head_dim = head_dim, p.pages = page_count, p.table_stride = table_stride;
-    p.page_shift = 4;
-    while ((1u << p.page_shift) < page_tokens) ++p.page_shift;
-    p.causal = causal != 0, p.q_bf16 = precision == 1, p.out_kind = output_precision;
-    p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    const Plan n = plan_rows(sequences, queries, true, max_length, p.group, kv_heads, kPlanSms);
-    DAV2_REQUIRE(n.slots <= 0x7FFFFFFFu, "cache attention: too many queries or sequences");
-    const uint64_t need = workspace_of(n, queries, q_heads, head_dim);
-    DAV2_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "cache attention: workspace is too small");
-    p.err = device_error_word();
-    if (!p.err) return set_error(DAV2CUDA_INTERNAL_ERROR, "cache attention: no device error word");
-    return run_rows(p, n, true, false, queries, workspace, as_stream(stream));
-}
-
-extern "C" DAV2CUDA_API uint64_t dav2cuda_cross_attention_16_workspace_size(uint32_t batch, uint32_t queries,
-                                                                            uint32_t keys, uint32_t q_heads,
-                                                                            uint32_t kv_heads, uint32_t head_dim) {
-    if (!batch || !queries || !shape_ok(q_heads, kv_heads)) return 0;
-    const Plan n = plan_rows(batch, queries, false, keys, q_heads / kv_heads, kv_heads, kPlanSms);
-    return workspace_of(n, (uint64_t)batch * queries, q_heads, head_dim);
-}
-
-extern "C" DAV2CUDA_API int dav2cuda_cross_attention_16(
-    void* output, const void* q, const void* k, const void* v, const int32_t* key_lengths, uint32_t batch,
-    uint32_t queries, uint32_t keys, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint64_t q_batch_stride,
-    uint64_t q_stride, uint64_t k_batch_stride, uint64_t k_stride, uint64_t v_batch_stride, uint64_t v_stride,
-    uint64_t output_batch_stride, uint64_t output_stride, float scale, uint32_t precision, uint32_t output_precision,
-    void* workspace, uint64_t workspace_bytes, void* stream) {
-    DAV2_REQUIRE(precision == 1 || precision == 2, "cross attention: operands must be bf16 or f16");
-    DAV2_REQUIRE(output_precision == 0 || output_precision == precision,
-                 "cross attention: output must be f32 or of the operands' type");
-    DAV2_REQUIRE(shape_ok(q_heads, kv_heads), "cross attention: q_heads must be a multiple of kv_heads");
-    DAV2_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0,
-                 "cross attention: head_dim must be a multiple of 8, 8 to 128");
-    DAV2_REQUIRE(std::isfinite(scale), "cross attention: invalid scale");
-    DAV2_REQUIRE((uint64_t)batch * queries * (q_heads / kv_heads) <= 0x3FFFFFFFu && keys <= 0x7FFFFF00u,
-                 "cross attention: too many queries or keys");
-    if (!queries || !batch) return DAV2CUDA_OK;
-    const uint64_t row = (uint64_t)q_heads * head_dim, kv_row = (uint64_t)kv_heads * head_dim;
-    DAV2_REQUIRE(queries == 1 || (q_stride >= row && output_stride >= row),
-                 "cross attention: a token stride is below the row of its heads");
-    DAV2_REQUIRE(keys <= 1 || (k_stride >= kv_row && v_stride >= kv_row),
-                 "cross attention: a token stride is below the row of its heads");
-    DAV2_REQUIRE(batch == 1 || output_batch_stride >= (queries - 1) * output_stride + row,
-                 "cross attention: output batches overlap");
-    DAV2_REQUIRE(!any_null(output, q) && (keys == 0 || !any_null(k, v)), "cross attention: null buffer");
-    DAV2_REQUIRE(aligned16(output) && aligned16(q) && aligned16(k) && aligned16(v) &&
-                     (queries == 1 || (q_stride % 8 == 0 && output_stride % 8 == 0)) &&
-                     (keys <= 1 || (k_stride % 8 == 0 && v_stride % 8 == 0)) &&
-                     (batch == 1 || (q_batch_stride % 8 == 0 && output_batch_stride % 8 == 0 &&
-                                     k_batch_stride % 8 == 0 && v_batch_stride % 8 == 0)),
-                 "cross attention: rows must be 16-byte aligned");
-    RowsParams p{};
-    p.out = output, p.q = q, p.k = k, p.v = v, p.lengths = key_lengths;
-    p.q_batch = q_batch_stride, p.q_stride = q_stride, p.k_batch = k_batch_stride, p.k_stride = k_stride;
-    p.v_batch = v_batch_stride, p.v_stride = v_stride, p.out_batch = output_batch_stride, p.out_stride = output_stride;
-    p.sequences = batch, p.queries = queries, p.max_length = keys, p.group = q_heads / kv_heads;
-    p.kv_heads = kv_heads, p.head_dim = head_dim, p.q_bf16 = precision == 1, p.out_kind = output_precision;
-    p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    const Plan n = plan_rows(batch, queries, false, keys, p.group, kv_heads, kPlanSms);
-    DAV2_REQUIRE(n.slots <= 0x7FFFFFFFu, "cross attention: too many queries");
-    const uint64_t tokens = (uint64_t)batch * queries, need = workspace_of(n, tokens, q_heads, head_dim);
-    DAV2_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "cross attention: workspace is too small");
-    p.err = device_error_word();
-    if (!p.err) return set_error(DAV2CUDA_INTERNAL_ERROR, "cross attention: no device error word");
-    return run_rows(p, n, false, precision == 1, tokens, workspace, as_stream(stream));
-}
