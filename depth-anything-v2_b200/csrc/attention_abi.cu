@@ -16,14 +16,15 @@ struct Plan {
     uint32_t row_tiles;  // 8-row tiles of a warp (rows kernel)
     uint32_t row_warps;  // row tiles of a block (rows kernel); 0: the tiles kernel
     uint32_t splits;     // of the keys
+    bool clusters;       // whose splits join in a cluster, not in the workspace
     uint64_t slots;      // row blocks over all sequences
 };
 
 #ifndef DAV2_TILES_FROM
 #define DAV2_TILES_FROM 33
 #endif
-// Rows that share a key head decide the kernel. Keys are split where the row
-// blocks alone would leave SMs idle, down to 256 keys to a block.
+// Rows that share a key head decide the kernel. Keys are split where the row blocks
+// alone would leave SMs idle, down to 128 keys (tiles kernel: 256) to a block.
 Plan plan_rows(uint64_t sequences, uint64_t queries, bool ragged, uint32_t max_length, uint32_t group,
                uint32_t kv_heads) {
     Plan n;
@@ -35,21 +36,32 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool ragged, uint32_t max_l
     const uint64_t tile = n.row_warps ? 8ull * n.row_tiles * n.row_warps : 256;
     n.slots = ragged ? queries * group / tile + sequences : sequences * ((rows + tile - 1) / tile);
     const uint64_t live = std::max<uint64_t>(1, sequences * ((rows + tile - 1) / tile)) * kv_heads;
-    const uint64_t want = n.row_warps ? (3ull * kSms + live - 1) / live : kSms / live;
-    const uint64_t most = std::max<uint64_t>(1, max_length / 256);
-    n.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(want, most), 128));
+    n.clusters = false;
+    if (!n.row_warps) {
+        n.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kSms / live, max_length / 256));
+        return n;
+    }
+    // The rows kernel: three blocks fit an SM. One sequence: as many equal splits as
+    // fill them once. Several, whose lengths may differ: about four times as many
+    // blocks as fit, so that the last ones even out. Up to eight splits are a cluster.
+    const uint64_t fit = 3ull * kSms, most = std::max<uint64_t>(1, max_length / 128);
+    uint64_t splits = sequences == 1 ? std::max<uint64_t>(1, fit / live) : (4 * fit + live - 1) / live;
+    if (splits > 8 && (live * 8 >= fit || max_length <= 8 * 1024)) splits = 8;
+    n.splits = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(splits, most), 128);
+    n.clusters = n.splits > 1 && n.splits <= 8;
     return n;
 }
 
 uint64_t workspace_of(const Plan& n, uint64_t tokens, uint32_t heads, uint32_t head_dim) {
-    if (n.splits == 1) return 0;
+    if (n.splits == 1 || n.clusters) return 0;
     return tokens * heads * n.splits * (head_dim * 4ull + 8) + 256;
 }
 
 int run(RowsParams& p, const Plan& n, bool s8, bool bf16, uint64_t tokens, void* workspace, cudaStream_t st) {
-    p.row_warps = n.row_warps, p.splits = n.splits;
+    p.row_warps = n.row_warps, p.splits = n.splits, p.clusters = n.clusters;
     const uint64_t rows = tokens * p.kv_heads * p.group;
-    if (n.splits > 1) {
+    const bool parts = n.splits > 1 && !n.clusters;
+    if (parts) {
         uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(workspace) + 15) & ~uintptr_t(15));
         p.part_o = reinterpret_cast<float*>(base);
         p.part_ml = reinterpret_cast<float2*>(base + rows * n.splits * p.head_dim * 4);
@@ -57,7 +69,7 @@ int run(RowsParams& p, const Plan& n, bool s8, bool bf16, uint64_t tokens, void*
     if (int rc = n.row_warps ? launch_attention_rows(p, (uint32_t)n.slots, n.row_tiles, s8, bf16, st)
                              : launch_attention_tiles(p, (uint32_t)n.slots, s8, bf16, st))
         return rc;
-    return n.splits > 1 ? launch_attention_join(p, rows, st) : DAV2CUDA_OK;
+    return parts ? launch_attention_join(p, rows, st) : DAV2CUDA_OK;
 }
 
 bool shape_ok(uint32_t q_heads, uint32_t kv_heads) {

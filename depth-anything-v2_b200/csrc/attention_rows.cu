@@ -29,7 +29,7 @@
 // the unrounded values. 16-bit values take p in their own type, as the tensor
 // core wants both operands alike.
 //
-// A block's four warps take either the same rows and every fourth 32 keys, merged
+// A block's four warps take either the same rows and every fourth step of keys, merged
 // at the end in shared memory, or (many rows) four row tiles and the same keys, which
 // they then find in L1. Where there are few row tiles, the keys of a tile are split
 // over several blocks whose (o, m, sum) go to the workspace, and a second kernel joins them.
@@ -40,7 +40,6 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
-constexpr uint32_t kChunk = 32;   // keys of one step of a warp
 constexpr float kRaise = 8.0f;    // m is raised when a score exceeds it by this
 
 template <bool kBF16>
@@ -62,121 +61,186 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-// One 16-key tile of codes or of 16-bit rows in registers.
-template <int D, bool kS8>
-struct Tile {
-    static constexpr int kK = kS8 ? D / 64 : D / 32;                 // 16-byte loads of a K row
-    static constexpr int kV = kS8 ? (D == 128 ? 4 : 2) : D / 16;     // words of a V row
-    uint4 k[2][kK];
-    uint32_t v[4][kV];
-    float sk, sv;
-    bool dead;  // no page of the cache: its keys are left out
-};
-
-struct Where {
-    uint32_t seq, kv_head, len;   // len: keys of the sequence
-};
-
-template <int D, bool kS8>
-__device__ __forceinline__ void load_tile(Tile<D, kS8>& f, const RowsParams& p, const Where& w, uint32_t key0,
-                                          uint32_t lane) {
-    const uint32_t g = lane >> 2, t = lane & 3, d = p.head_dim;
-    const uint32_t kr = key0 + 4 * (g >> 1) + (g & 1);  // S^T row g is key kr, row g + 8 key kr + 2
-    f.dead = false;
-    if constexpr (kS8) {
-        f.sk = f.sv = 0.0f;
-        int32_t page = -1;
-        if (key0 < w.len) {
-            page = p.page_table[(uint64_t)w.seq * p.table_stride + (key0 >> p.page_shift)];
-            if (page < 0 || (uint32_t)page >= p.pages) {
-                if (lane == 0) atomicExch(p.err, 3);
-                page = -1;
-            }
-        }
-        if (page < 0) {
-            f.dead = true;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < f.kK; ++i) f.k[h][i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < f.kV; ++j) f.v[i][j] = 0;
-            return;
-        }
-        const uint64_t unit = (uint64_t)page * p.kv_heads + w.kv_head;
-        f.sk = p.k_scales[unit], f.sv = p.v_scales[unit];
-        const uint32_t in_page = (1u << p.page_shift) - 1;
-        const uint64_t base = (unit << p.page_shift) * d;
-        const int8_t* k = static_cast<const int8_t*>(p.k) + base;
-        const int8_t* v = static_cast<const int8_t*>(p.v) + base;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < f.kK; ++i) {
-                const uint32_t at = 64 * i + 16 * t;
-                f.k[h][i] = at < d ? *reinterpret_cast<const uint4*>(k + ((kr + 2 * h) & in_page) * d + at)
-                                   : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int8_t* row = v + ((key0 + 4 * t + i) & in_page) * d;
-            if constexpr (D == 128) {
-                const uint4 x = 16 * g < d ? *reinterpret_cast<const uint4*>(row + 16 * g) : make_uint4(0, 0, 0, 0);
-                f.v[i][0] = x.x, f.v[i][1] = x.y, f.v[i][2] = x.z, f.v[i][3] = x.w;
-            } else {
-                const uint2 x = 8 * g < d ? *reinterpret_cast<const uint2*>(row + 8 * g) : make_uint2(0, 0);
-                f.v[i][0] = x.x, f.v[i][1] = x.y;
-            }
-        }
-    } else {
-        f.sk = f.sv = 1.0f;
-        const uint16_t* k = static_cast<const uint16_t*>(p.k) + w.seq * p.k_batch + (uint64_t)w.kv_head * d;
-        const uint16_t* v = static_cast<const uint16_t*>(p.v) + w.seq * p.v_batch + (uint64_t)w.kv_head * d;
-        // rows past the end are not read: they may be no memory, or hold NaN
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < f.kK; ++i) {
-                const uint32_t at = 32 * i + 8 * t, key = kr + 2 * h;
-                f.k[h][i] = at < d && key < w.len
-                                ? *reinterpret_cast<const uint4*>(k + key * p.k_stride + at)
-                                : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < f.kV; j += 4) {
-                const uint32_t at = D / 8 * g + 2 * j, key = key0 + 4 * t + i;
-                const uint4 x = at < d && key < w.len ? *reinterpret_cast<const uint4*>(v + key * p.v_stride + at)
-                                                      : make_uint4(0, 0, 0, 0);
-                f.v[i][j] = x.x, f.v[i][j + 1] = x.y, f.v[i][j + 2] = x.z, f.v[i][j + 3] = x.w;
-            }
-    }
-}
-
 __device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Address of a shared-memory place of this block in another block of the cluster.
+__device__ __forceinline__ uint32_t cluster_place(const void* p, uint32_t rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+
+__device__ __forceinline__ float cluster_load(uint32_t place) {
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(place) : "memory");
+    return x;
+}
+
+__device__ __forceinline__ float2 cluster_load2(uint32_t place) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(place) : "memory");
+    return x;
+}
+
+// The keys of one step of a warp in registers, as tiles of 16 (4 KB of codes or of
+// 16-bit values at D = 128, K and V). S^T's row g of a tile is key 4 (g / 2) + g % 2, row g + 8 the second next; a lane's V rows are keys 4t .. 4t + 3.
+// kFull: head_dim == D, known to the compiler.
+template <int D, bool kS8, bool kFull>
+struct Source {
+    static constexpr int kTiles = kS8 ? 2 : 1;
+    static constexpr uint32_t kChunk = 16 * kTiles;
+    static constexpr int kK = kS8 ? D / 64 : D / 32;              // 16-byte loads of a K row
+    static constexpr int kV = kS8 ? (D == 128 ? 4 : 2) : D / 16;  // words of a V row
+    const RowsParams& p;
+    uint32_t seq, kv_head, len, g, t, d;
+    uint64_t at_k, at_v;                // this lane's place in a tile, 16-bit rows: in the batch entry
+    uint4 k[kTiles][2][kK];                  // [tile][row][load]
+    uint32_t v[kTiles][4][kV];          // [tile][key][word]
+    float sk[kTiles], sv[kTiles];
+    int32_t page_k[kTiles], page_v[kTiles], page_next[kTiles];  // of the tiles in k, in v, and of the chunk to come; -1: none
+
+    __device__ Source(const RowsParams& p, uint32_t seq, uint32_t kv_head, uint32_t len, uint32_t lane)
+        : p(p), seq(seq), kv_head(kv_head), len(len), g(lane >> 2), t(lane & 3), d(kFull ? D : p.head_dim) {
+        const uint32_t kr = 4 * (g >> 1) + (g & 1);
+        if constexpr (kS8) {
+            at_k = kr * d + 16 * t;
+            at_v = 4 * t * d + D / 8 * g;
+        } else {
+            at_k = seq * p.k_batch + (uint64_t)kv_head * d + kr * p.k_stride + 8 * t;
+            at_v = seq * p.v_batch + (uint64_t)kv_head * d + 4 * t * p.v_stride + D / 8 * g;
+        }
+    }
+
+    // The pages of the chunk at key0 (codes), fetched ahead of their use.
+    __device__ __forceinline__ void fetch_pages(uint32_t key0) {
+        if constexpr (kS8) {
+#pragma unroll
+            for (int b = 0; b < kTiles; ++b) {
+                const uint32_t key = key0 + 16 * b;
+                page_next[b] =
+                    key < len ? p.page_table[(uint64_t)seq * p.table_stride + (key >> p.page_shift)] : -1;
+            }
+        }
+    }
+
+    __device__ __forceinline__ uint64_t tile_of(int32_t page, uint32_t key) const {
+        const uint64_t unit = (uint64_t)(uint32_t)page * p.kv_heads + kv_head;
+        return ((unit << p.page_shift) + (key & ((1u << p.page_shift) - 1))) * d;
+    }
+
+    __device__ __forceinline__ void load_k(uint32_t key0) {
+        if constexpr (kS8) {
+#pragma unroll
+            for (int b = 0; b < kTiles; ++b) {
+                const uint32_t key = key0 + 16 * b;
+                int32_t page = page_next[b];
+                if (page < 0 || (uint32_t)page >= p.pages) {
+                    if (key < len && threadIdx.x % 32 == 0) atomicExch(p.err, 3);
+                    page = -1;
+                }
+                page_k[b] = page;
+                sk[b] = sv[b] = 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < kK; ++i) k[b][h][i] = make_uint4(0, 0, 0, 0);
+                if (page < 0) continue;
+                const uint64_t unit = (uint64_t)(uint32_t)page * p.kv_heads + kv_head;
+                sk[b] = p.k_scales[unit], sv[b] = p.v_scales[unit];
+                const int8_t* from = static_cast<const int8_t*>(p.k) + tile_of(page, key) + at_k;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < kK; ++i)
+                        if (kFull || 64 * i + 16 * t < d)
+                            k[b][h][i] = *reinterpret_cast<const uint4*>(from + 2 * h * d + 64 * i);
+            }
+        } else {
+            // rows past the end are not read: they may be no memory, or hold NaN
+            const uint16_t* from = static_cast<const uint16_t*>(p.k) + at_k + key0 * p.k_stride;
+            const uint32_t key = key0 + 4 * (g >> 1) + (g & 1);
+#pragma unroll
+            for (int b = 0; b < kTiles; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < kK; ++i)
+                        k[b][h][i] = (kFull || 32 * i + 8 * t < d) && key + 16 * b + 2 * h < len
+                                         ? *reinterpret_cast<const uint4*>(from + (16 * b + 2 * h) * p.k_stride + 32 * i)
+                                         : make_uint4(0, 0, 0, 0);
+        }
+    }
+
+    __device__ __forceinline__ void load_v(uint32_t key0) {
+        if constexpr (kS8) {
+#pragma unroll
+            for (int b = 0; b < kTiles; ++b) {
+                page_v[b] = page_k[b];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kV; ++j) v[b][i][j] = 0;
+                if (page_v[b] < 0 || !(kFull || D / 8 * g < d)) continue;
+                const int8_t* from = static_cast<const int8_t*>(p.v) + tile_of(page_v[b], key0 + 16 * b) + at_v;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (D == 128) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(from + i * d);
+                        v[b][i][0] = x.x, v[b][i][1] = x.y, v[b][i][2] = x.z, v[b][i][3] = x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(from + i * d);
+                        v[b][i][0] = x.x, v[b][i][1] = x.y;
+                    }
+                }
+            }
+        } else {
+            const uint16_t* from = static_cast<const uint16_t*>(p.v) + at_v + key0 * p.v_stride;
+#pragma unroll
+            for (int b = 0; b < kTiles; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < kV; j += 4) {
+                        const uint4 x = (kFull || D / 8 * g + 2 * j < d) && key0 + 16 * b + 4 * t + i < len
+                                            ? *reinterpret_cast<const uint4*>(from + (16 * b + i) * p.v_stride + 2 * j)
+                                            : make_uint4(0, 0, 0, 0);
+                        v[b][i][j] = x.x, v[b][i][j + 1] = x.y, v[b][i][j + 2] = x.z, v[b][i][j + 3] = x.w;
+                    }
+        }
+    }
+};
+
 // kBF16: type of the second product's operands (false for codes).
-template <int D, int NT, bool kS8, bool kBF16>
+template <int D, int NT, bool kS8, bool kBF16, bool kFull>
 __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsParams p) {
-    constexpr int kSteps = D / 16;
+    using Keys = Source<D, kS8, kFull>;
+    constexpr int kSteps = D / 16, kTiles = Keys::kTiles;
+    constexpr uint32_t kChunk = Keys::kChunk;
     constexpr int R = 8 * NT;
     __shared__ float s_o[kWarps][R][D + 4];
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+    __shared__ float c_m[kWarps * R], c_l[kWarps * R];  // of the block's rows, for the cluster
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint32_t tile_rows = R * p.row_warps, key_warps = kWarps / p.row_warps;
     const uint32_t row_warp = warp / key_warps, key_warp = warp % key_warps;
+    const uint32_t d = kFull ? D : p.head_dim;
 
     RowTile where;
     if (!find_row_tile(where, p, blockIdx.x, tile_rows)) return;
-    Where w;
-    w.kv_head = blockIdx.y;
-    w.seq = where.seq;
-    w.len = keys_of(p, where.seq);
-    const uint32_t rows = where.rows;
+    const uint32_t kv_head = blockIdx.y, len = keys_of(p, where.seq), rows = where.rows;
     const uint32_t row0 = where.tile * tile_rows + row_warp * R;  // this warp's first row
+
+    // the keys of this split, in steps of kChunk, every key_warps-th for this warp
+    const uint32_t chunks = (len + kChunk - 1) / kChunk;
+    const uint32_t per_split = (chunks + p.splits - 1) / p.splits;
+    const uint32_t first = blockIdx.z * per_split;
+    Keys f(p, where.seq, kv_head, len, lane);
+    uint32_t c = first + key_warp;
+    f.fetch_pages(c * kChunk);
 
     // q as the products' B fragments, and the factors of its rows
     uint32_t qf[NT][kSteps][2];
@@ -185,14 +249,15 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t row = row0 + 8 * n + g;
-        const uint16_t* q = static_cast<const uint16_t*>(p.q) + (row < rows ? row_at(p, where, w.kv_head, row, p.q_batch, p.q_stride) : 0);
+        const uint16_t* q = static_cast<const uint16_t*>(p.q) +
+                            (row < rows ? row_at(p, where, kv_head, row, p.q_batch, p.q_stride) : 0);
         float most = 0.0f;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
             // the dims of k-step j that the lane's K bytes hold
             const uint32_t at = kS8 ? 64 * (j / 4) + 16 * t + 4 * (j % 4) : 32 * (j / 2) + 8 * t + 4 * (j % 2);
             uint2 x = make_uint2(0, 0);
-            if (row < rows && at < p.head_dim) x = *reinterpret_cast<const uint2*>(q + at);
+            if (row < rows && at < d) x = *reinterpret_cast<const uint2*>(q + at);
             qf[n][j][0] = x.x, qf[n][j][1] = x.y;
             if constexpr (kS8) {
                 const float2 a = unpack2(x.x, p.q_bf16), b = unpack2(x.y, p.q_bf16);
@@ -221,7 +286,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             factor[n][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e)) * p.scale_log2;
-            reach[n][e] = reach_of(p, where, w.len, row0 + 8 * n + 2 * t + e);
+            reach[n][e] = reach_of(p, where, len, row0 + 8 * n + 2 * t + e);
             low = min(low, reach[n][e]);
             high = max(high, reach[n][e]);
         }
@@ -231,11 +296,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
         high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
     }
-
-    // the keys of this split, in steps of kChunk, every key_warps-th for this warp
-    const uint32_t chunks = (w.len + kChunk - 1) / kChunk;
-    const uint32_t per_split = (chunks + p.splits - 1) / p.splits;
-    const uint32_t first = blockIdx.z * per_split, last = min(chunks, first + per_split);
+    const uint32_t last = min(min(chunks, first + per_split), (high + kChunk - 1) / kChunk);
 
     float o[kSteps][NT][4], m[NT][2], l[NT][2], ref = 1e-30f, inv_ref = 128.0f / 1e-30f;
 #pragma unroll
@@ -246,22 +307,26 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         l[n][0] = l[n][1] = 0.0f;
     }
 
-    for (uint32_t c = first + key_warp; c < last; c += key_warps) {
-        const uint32_t key0 = c * kChunk;
-        if (key0 >= high) break;
-        Tile<D, kS8> f[2];
-        load_tile<D, kS8>(f[0], p, w, key0, lane);
-        load_tile<D, kS8>(f[1], p, w, key0 + 16, lane);
-        float sc[2][NT][4];
+    // Two loads are in flight at any time: K of the next chunk from the first product
+    // on, V of the next chunk from the second on, into the registers just used.
+    if (c < last) {
+        f.load_k(c * kChunk);
+        f.load_v(c * kChunk);
+        f.fetch_pages((c + key_warps) * kChunk);
+    }
+    for (; c < last; c += key_warps) {
+        const uint32_t key0 = c * kChunk, next = (c + key_warps) * kChunk;
+        const bool more = c + key_warps < last;
+        float sc[kTiles][NT][4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kTiles; ++b) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) sc[b][n][0] = sc[b][n][1] = sc[b][n][2] = sc[b][n][3] = 0.0f;
             if constexpr (kS8) {
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j) {
-                    const uint32_t x = word(f[b].k[0][j / 4], j % 4) ^ 0x80808080u;
-                    const uint32_t y = word(f[b].k[1][j / 4], j % 4) ^ 0x80808080u;
+                    const uint32_t x = word(f.k[b][0][j / 4], j % 4) ^ 0x80808080u;
+                    const uint32_t y = word(f.k[b][1][j / 4], j % 4) ^ 0x80808080u;
                     const uint32_t a0 = codes_lo(x), a1 = codes_lo(y), a2 = codes_hi(x), a3 = codes_hi(y);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_16816<false>(sc[b][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
@@ -269,7 +334,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             } else {
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j) {
-                    const uint4 &x = f[b].k[0][j / 2], &y = f[b].k[1][j / 2];
+                    const uint4 &x = f.k[b][0][j / 2], &y = f.k[b][1][j / 2];
                     const int i = 2 * (j % 2);
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -278,33 +343,43 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                 }
             }
         }
+        float sk[kTiles], sv[kTiles], sv_top = 0.0f;
+        bool dead[kTiles], any_dead = false;
+#pragma unroll
+        for (int b = 0; b < kTiles; ++b) {
+            sk[b] = kS8 ? f.sk[b] : 1.0f, sv[b] = kS8 ? f.sv[b] : 1.0f;
+            sv_top = fmaxf(sv_top, sv[b]);
+            dead[b] = kS8 && f.page_k[b] < 0;
+            any_dead |= dead[b];
+        }
+        if (more) f.load_k(next);
         // scores in units of log2, the keys out of reach at -inf
         bool raise = false;
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < kTiles; ++b)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[b][n][e] *= factor[n][e & 1] * f[b].sk;
-        if (key0 + kChunk > low || f[0].dead || f[1].dead) {
+                for (int e = 0; e < 4; ++e) sc[b][n][e] *= kS8 ? factor[n][e & 1] * sk[b] : factor[n][e & 1];
+        if (key0 + kChunk > low || any_dead) {
             const uint32_t key = key0 + 4 * (g >> 1) + (g & 1);
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < kTiles; ++b)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (f[b].dead || key + 16 * b + (e >= 2 ? 2 : 0) >= reach[n][e & 1]) sc[b][n][e] = -INFINITY;
+                        if (dead[b] || key + 16 * b + (e >= 2 ? 2 : 0) >= reach[n][e & 1]) sc[b][n][e] = -INFINITY;
         }
         float top[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                top[n][e] = fmaxf(fmaxf(sc[0][n][e], sc[0][n][e + 2]), fmaxf(sc[1][n][e], sc[1][n][e + 2]));
+                top[n][e] = fmaxf(sc[0][n][e], sc[0][n][e + 2]);
+                if (kTiles == 2) top[n][e] = fmaxf(top[n][e], fmaxf(sc[kTiles - 1][n][e], sc[kTiles - 1][n][e + 2]));
                 raise |= top[n][e] > m[n][e] + kRaise;
             }
-        const float sv_top = fmaxf(f[0].sv, f[1].sv);
         if (__any_sync(0xffffffffu, raise) || (kS8 && sv_top > ref)) {
             float unit = 1.0f;
             if (kS8 && sv_top > ref) {
@@ -327,10 +402,10 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                     for (int i = 0; i < kSteps; ++i) o[i][n][e] *= down * unit, o[i][n][e + 2] *= down * unit;
                 }
         }
-        uint32_t pf[2][NT][2];
+        uint32_t pf[kTiles][NT][2];
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const float weight = kS8 ? f[b].sv * inv_ref : kBF16 ? 1.0f : 128.0f;
+        for (int b = 0; b < kTiles; ++b) {
+            const float weight = kS8 ? sv[b] * inv_ref : kBF16 ? 1.0f : 128.0f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float e4[4];
@@ -346,11 +421,11 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             }
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-            const auto& v = f[b].v;
+        for (int b = 0; b < kTiles; ++b) {
+            const auto& v = f.v[b];
             if constexpr (kS8) {
 #pragma unroll
-                for (int i = 0; i < f[0].kV; ++i) {
+                for (int i = 0; i < f.kV; ++i) {
                     const uint32_t x0 = v[0][i] ^ 0x80808080u, x1 = v[1][i] ^ 0x80808080u;
                     const uint32_t x2 = v[2][i] ^ 0x80808080u, x3 = v[3][i] ^ 0x80808080u;
                     const uint32_t l01 = prmt(x0, x1, 0x5140), h01 = prmt(x0, x1, 0x7362);
@@ -365,13 +440,17 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < f[0].kV; ++i) {
+                for (int i = 0; i < f.kV; ++i) {
                     const uint32_t a0 = prmt(v[0][i], v[1][i], 0x5410), a1 = prmt(v[0][i], v[1][i], 0x7632);
                     const uint32_t a2 = prmt(v[2][i], v[3][i], 0x5410), a3 = prmt(v[2][i], v[3][i], 0x7632);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_16816<kBF16>(o[i][n], a0, a1, a2, a3, pf[b][n][0], pf[b][n][1]);
                 }
             }
+        }
+        if (more) {
+            f.load_v(next);
+            f.fetch_pages(next + key_warps * kChunk);
         }
     }
 
@@ -394,31 +473,58 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     __syncthreads();
 
     // merge the key warps of each row tile: a thread takes two dims of a row
-    for (uint32_t i = threadIdx.x; i < R * p.row_warps * (D / 2); i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < tile_rows * (D / 2); i += kThreads) {
         const uint32_t r = i / (D / 2), dim = 2 * (i - r * (D / 2));
-        const uint32_t rw = r / R, col = r - rw * R, row = where.tile * tile_rows + r;
-        if (row >= rows || dim >= p.head_dim) continue;
+        const uint32_t w0 = r / R * key_warps, col = r % R, row = where.tile * tile_rows + r;
+        if (row >= rows || dim >= d) continue;
         float top = -INFINITY;
-        for (uint32_t k = 0; k < key_warps; ++k) top = fmaxf(top, s_m[rw * key_warps + k][col]);
+        for (uint32_t k = 0; k < key_warps; ++k) top = fmaxf(top, s_m[w0 + k][col]);
         float sum = 0.0f, x[2] = {0.0f, 0.0f};
         for (uint32_t k = 0; k < key_warps; ++k) {
-            const uint32_t kw = rw * key_warps + k;
-            if (s_m[kw][col] == -INFINITY) continue;
-            const float a = ex2_approx(s_m[kw][col] - top);
-            sum += a * s_l[kw][col];
-            x[0] += a * s_o[kw][col][dim];
-            x[1] += a * s_o[kw][col][dim + 1];
+            if (s_m[w0 + k][col] == -INFINITY) continue;
+            const float a = ex2_approx(s_m[w0 + k][col] - top);
+            sum += a * s_l[w0 + k][col];
+            const float2 b = *reinterpret_cast<const float2*>(&s_o[w0 + k][col][dim]);
+            x[0] += a * b.x;
+            x[1] += a * b.y;
         }
         if (p.splits == 1) {
             const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
             x[0] *= inv, x[1] *= inv;
-            store_out(p, row_at(p, where, w.kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
+            store_out(p, row_at(p, where, kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
+        } else if (p.clusters) {
+            *reinterpret_cast<float2*>(&s_o[w0][col][dim]) = make_float2(x[0], x[1]);  // read by this thread alone
+            if (dim == 0) c_m[r] = top, c_l[r] = sum;
         } else {
-            const uint64_t slot = part_at(p, where, w.kv_head, row, blockIdx.z);
+            const uint64_t slot = part_at(p, where, kv_head, row, blockIdx.z);
             if (dim == 0) p.part_ml[slot] = make_float2(top, sum);
-            if (sum > 0.0f) *reinterpret_cast<float2*>(p.part_o + slot * p.head_dim + dim) = make_float2(x[0], x[1]);
+            if (sum > 0.0f) *reinterpret_cast<float2*>(p.part_o + slot * d + dim) = make_float2(x[0], x[1]);
         }
     }
+    if (!p.clusters) return;
+    // the splits are a cluster: each block merges its share of the rows' dims
+    cluster_sync();
+    for (uint32_t i = blockIdx.z * kThreads + threadIdx.x; i < tile_rows * (D / 2); i += p.splits * kThreads) {
+        const uint32_t r = i / (D / 2), dim = 2 * (i - r * (D / 2));
+        const uint32_t w0 = r / R * key_warps, col = r % R, row = where.tile * tile_rows + r;
+        if (row >= rows || dim >= d) continue;
+        float top = -INFINITY;
+        for (uint32_t k = 0; k < p.splits; ++k) top = fmaxf(top, cluster_load(cluster_place(&c_m[r], k)));
+        float sum = 0.0f, x[2] = {0.0f, 0.0f};
+        for (uint32_t k = 0; k < p.splits; ++k) {
+            const float mk = cluster_load(cluster_place(&c_m[r], k));
+            if (mk == -INFINITY) continue;
+            const float a = ex2_approx(mk - top);
+            sum += a * cluster_load(cluster_place(&c_l[r], k));
+            const float2 b = cluster_load2(cluster_place(&s_o[w0][col][dim], k));
+            x[0] += a * b.x;
+            x[1] += a * b.y;
+        }
+        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        x[0] *= inv, x[1] *= inv;
+        store_out(p, row_at(p, where, kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
+    }
+    cluster_sync();  // no block leaves while another reads its shared memory
 }
 
 // Joins the splits of each row: a warp to a row.
@@ -457,26 +563,39 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const RowsPara
     if (dim < p.head_dim) store_out(p, (p.query_begin ? flat : at) + dim, x, 4);
 }
 
+template <int D, int NT, bool kS8, bool kBF16, bool kFull>
+int start(const RowsParams& p, uint32_t slots, cudaStream_t st) {
+    cudaLaunchAttribute cluster[1];
+    cluster[0].id = cudaLaunchAttributeClusterDimension;
+    cluster[0].val.clusterDim.x = 1, cluster[0].val.clusterDim.y = 1, cluster[0].val.clusterDim.z = p.splits;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(slots, p.kv_heads, p.splits);
+    config.blockDim = dim3(kThreads);
+    config.stream = st;
+    config.attrs = cluster;
+    config.numAttrs = p.clusters ? 1 : 0;
+    cudaLaunchKernelEx(&config, attention_rows_kernel<D, NT, kS8, kBF16, kFull>, p);
+    return check_launch("attention_rows");
+}
+
 template <bool kS8, bool kBF16>
-void start_for(const RowsParams& p, uint32_t slots, uint32_t row_tiles, cudaStream_t st) {
-    const dim3 grid(slots, p.kv_heads, p.splits);
-    if (p.head_dim <= 64) {
-        if (row_tiles == 1) attention_rows_kernel<64, 1, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
-        else attention_rows_kernel<64, 2, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
-    } else {
-        if (row_tiles == 1) attention_rows_kernel<128, 1, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
-        else attention_rows_kernel<128, 2, kS8, kBF16><<<grid, kThreads, 0, st>>>(p);
-    }
+int start_for(const RowsParams& p, uint32_t slots, uint32_t row_tiles, cudaStream_t st) {
+    if (p.head_dim == 64) return row_tiles == 1 ? start<64, 1, kS8, kBF16, true>(p, slots, st)
+                                                : start<64, 2, kS8, kBF16, true>(p, slots, st);
+    if (p.head_dim == 128) return row_tiles == 1 ? start<128, 1, kS8, kBF16, true>(p, slots, st)
+                                                 : start<128, 2, kS8, kBF16, true>(p, slots, st);
+    if (p.head_dim < 64) return row_tiles == 1 ? start<64, 1, kS8, kBF16, false>(p, slots, st)
+                                               : start<64, 2, kS8, kBF16, false>(p, slots, st);
+    return row_tiles == 1 ? start<128, 1, kS8, kBF16, false>(p, slots, st)
+                          : start<128, 2, kS8, kBF16, false>(p, slots, st);
 }
 
 }  // namespace
 
 int launch_attention_rows(const RowsParams& p, uint32_t slots, uint32_t row_tiles, bool s8, bool bf16,
                           cudaStream_t st) {
-    if (s8) start_for<true, false>(p, slots, row_tiles, st);
-    else if (bf16) start_for<false, true>(p, slots, row_tiles, st);
-    else start_for<false, false>(p, slots, row_tiles, st);
-    return check_launch("attention_rows");
+    if (s8) return start_for<true, false>(p, slots, row_tiles, st);
+    return bf16 ? start_for<false, true>(p, slots, row_tiles, st) : start_for<false, false>(p, slots, row_tiles, st);
 }
 
 int launch_attention_join(const RowsParams& p, uint64_t rows, cudaStream_t st) {

@@ -18,8 +18,9 @@ struct RowsParams {
     const int32_t* query_begin;  // null: sequence s has rows [s * queries, (s + 1) * queries)
     uint64_t q_batch, q_stride, k_batch, k_stride, v_batch, v_stride, out_batch, out_stride;
     uint32_t sequences, queries, max_length, group, kv_heads, head_dim, pages, page_shift, table_stride;
-    uint32_t causal, row_warps, splits, q_bf16, out_kind;  // out_kind: 0 f32, 1 bf16, 2 f16
+    uint32_t causal, row_warps, splits, clusters, q_bf16, out_kind;  // out_kind: 0 f32, 1 bf16, 2 f16
     float scale_log2;
+    // clusters: the splits of a row tile are the blocks of a cluster and join there
     float* part_o;   // [query][head][split][head_dim]
     float2* part_ml; // [query][head][split]
     int* err;
