@@ -25,8 +25,9 @@ struct Plan {
 #endif
 // Rows that share a key head decide the kernel. Keys are split where the row blocks
 // alone would leave SMs idle, down to 128 keys (tiles kernel: 256) to a block.
-Plan plan_rows(uint64_t sequences, uint64_t queries, bool ragged, uint32_t max_length, uint32_t group,
-               uint32_t kv_heads) {
+Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_length, uint32_t group,
+               uint32_t kv_heads, uint32_t head_dim) {
+    const bool ragged = s8;  // query_begin gives the rows of a sequence
     Plan n;
     const uint64_t each = ragged ? (queries + sequences - 1) / sequences : queries;
     const uint64_t rows = each * group;
@@ -41,13 +42,16 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool ragged, uint32_t max_l
         n.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kSms / live, max_length / 256));
         return n;
     }
-    // The rows kernel: three blocks fit an SM. One sequence: as many equal splits as
-    // fill them once. Several, whose lengths may differ: about four times as many
-    // blocks as fit, so that the last ones even out. Up to eight splits are a cluster.
-    const uint64_t fit = 3ull * kSms, most = std::max<uint64_t>(1, max_length / 128);
-    uint64_t splits = sequences == 1 ? std::max<uint64_t>(1, fit / live) : (4 * fit + live - 1) / live;
-    if (splits > 8 && (live * 8 >= fit || max_length <= 8 * 1024)) splits = 8;
-    n.splits = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(splits, most), 128);
+    // The rows kernel. What fits the device at once is filled by one wave of equal
+    // splits; where lengths may differ and are long, about two waves even out the end
+    // (48 streams of up to 8192 keys: 1, 2, 3 splits 134, 118, 124 us). Up to eight
+    // splits are a cluster and join there, without the workspace and a second launch.
+    const uint64_t fit = (uint64_t)kSms * (s8 ? (head_dim <= 64 ? 6 : 3) : 2);
+    const uint64_t most = std::max<uint64_t>(1, max_length / 128);
+    uint64_t splits = std::max<uint64_t>(1, fit / live);
+    if (sequences > 1) splits = std::max(splits, std::min<uint64_t>((2 * fit + live - 1) / live, max_length / 4096));
+    if (splits > 8 && (live * 8 >= fit || max_length <= 4096)) splits = 8;
+    n.splits = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(splits, most), kMaxSplits);
     n.clusters = n.splits > 1 && n.splits <= 8;
     return n;
 }
@@ -85,7 +89,7 @@ extern "C" DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint
                                                                             uint32_t max_length, uint32_t q_heads,
                                                                             uint32_t kv_heads, uint32_t head_dim) {
     if (!sequences || !queries || !shape_ok(q_heads, kv_heads)) return 0;
-    const Plan n = plan_rows(sequences, queries, true, max_length, q_heads / kv_heads, kv_heads);
+    const Plan n = plan_rows(sequences, queries, true, max_length, q_heads / kv_heads, kv_heads, head_dim);
     return workspace_of(n, queries, q_heads, head_dim);
 }
 
@@ -129,7 +133,7 @@ extern "C" DAV2CUDA_API int dav2cuda_attention_cache_s8(
     while ((1u << p.page_shift) < page_tokens) ++p.page_shift;
     p.causal = causal != 0, p.q_bf16 = precision == 1, p.out_kind = output_precision;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    const Plan n = plan_rows(sequences, queries, true, max_length, p.group, kv_heads);
+    const Plan n = plan_rows(sequences, queries, true, max_length, p.group, kv_heads, head_dim);
     DAV2_REQUIRE(n.slots <= 0x7FFFFFFFu, "cache attention: too many queries or sequences");
     const uint64_t need = workspace_of(n, queries, q_heads, head_dim);
     DAV2_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "cache attention: workspace is too small");
@@ -142,7 +146,7 @@ extern "C" DAV2CUDA_API uint64_t dav2cuda_cross_attention_16_workspace_size(uint
                                                                             uint32_t keys, uint32_t q_heads,
                                                                             uint32_t kv_heads, uint32_t head_dim) {
     if (!batch || !queries || !shape_ok(q_heads, kv_heads)) return 0;
-    const Plan n = plan_rows(batch, queries, false, keys, q_heads / kv_heads, kv_heads);
+    const Plan n = plan_rows(batch, queries, false, keys, q_heads / kv_heads, kv_heads, head_dim);
     return workspace_of(n, (uint64_t)batch * queries, q_heads, head_dim);
 }
 
@@ -183,7 +187,7 @@ extern "C" DAV2CUDA_API int dav2cuda_cross_attention_16(
     p.sequences = batch, p.queries = queries, p.max_length = keys, p.group = q_heads / kv_heads;
     p.kv_heads = kv_heads, p.head_dim = head_dim, p.q_bf16 = precision == 1, p.out_kind = output_precision;
     p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-    const Plan n = plan_rows(batch, queries, false, keys, p.group, kv_heads);
+    const Plan n = plan_rows(batch, queries, false, keys, p.group, kv_heads, head_dim);
     DAV2_REQUIRE(n.slots <= 0x7FFFFFFFu, "cross attention: too many queries");
     const uint64_t tokens = (uint64_t)batch * queries, need = workspace_of(n, tokens, q_heads, head_dim);
     DAV2_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "cross attention: workspace is too small");

@@ -33,6 +33,8 @@
 // at the end in shared memory, or (many rows) four row tiles and the same keys, which
 // they then find in L1. Where there are few row tiles, the keys of a tile are split
 // over several blocks whose (o, m, sum) go to the workspace, and a second kernel joins them.
+#include <algorithm>
+
 #include "attention_rows.cuh"
 
 namespace dav2cuda {
@@ -41,6 +43,9 @@ namespace {
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
 constexpr float kRaise = 8.0f;    // m is raised when a score exceeds it by this
+// Where m starts: finite, so that -inf - m is -inf and rows that see nothing get p = 0
+// without a test; any finite score above it raises it.
+constexpr float kLowest = -3.402823466e38f;
 
 template <bool kBF16>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -86,40 +91,69 @@ __device__ __forceinline__ float2 cluster_load2(uint32_t place) {
     return x;
 }
 
-// The keys of one step of a warp in registers, as tiles of 16 (4 KB of codes or of
-// 16-bit values at D = 128, K and V). S^T's row g of a tile is key 4 (g / 2) + g % 2, row g + 8 the second next; a lane's V rows are keys 4t .. 4t + 3.
-// kFull: head_dim == D, known to the compiler.
-template <int D, bool kS8, bool kFull>
-struct Source {
-    static constexpr int kTiles = kS8 ? 2 : 1;
-    static constexpr uint32_t kChunk = 16 * kTiles;
-    static constexpr int kK = kS8 ? D / 64 : D / 32;              // 16-byte loads of a K row
-    static constexpr int kV = kS8 ? (D == 128 ? 4 : 2) : D / 16;  // words of a V row
-    const RowsParams& p;
-    uint32_t seq, kv_head, len, g, t, d;
-    uint64_t at_k, at_v;                // this lane's place in a tile, 16-bit rows: in the batch entry
-    uint4 k[kTiles][2][kK];                  // [tile][row][load]
-    uint32_t v[kTiles][4][kV];          // [tile][key][word]
-    float sk[kTiles], sv[kTiles];
-    int32_t page_k[kTiles], page_v[kTiles], page_next[kTiles];  // of the tiles in k, in v, and of the chunk to come; -1: none
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16u : 0u) : "memory");
+}
 
-    __device__ Source(const RowsParams& p, uint32_t seq, uint32_t kv_head, uint32_t len, uint32_t lane)
-        : p(p), seq(seq), kv_head(kv_head), len(len), g(lane >> 2), t(lane & 3), d(kFull ? D : p.head_dim) {
-        const uint32_t kr = 4 * (g >> 1) + (g & 1);
-        if constexpr (kS8) {
-            at_k = kr * d + 16 * t;
-            at_v = 4 * t * d + D / 8 * g;
-        } else {
-            at_k = seq * p.k_batch + (uint64_t)kv_head * d + kr * p.k_stride + 8 * t;
-            at_v = seq * p.v_batch + (uint64_t)kv_head * d + 4 * t * p.v_stride + D / 8 * g;
-        }
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ uint4 read16(uint32_t from) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(from) : "memory");
+    return x;
+}
+
+__device__ __forceinline__ uint2 read8(uint32_t from) {
+    uint2 x;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(from) : "memory");
+    return x;
+}
+
+// A warp's ring of 16-key tiles of K and V in shared memory, filled by asynchronous
+// 16-byte copies that the warp issues for itself: no other warp waits on it. Rows
+// are D values long; chunk c (16 bytes) of row r lies in 128-byte line (r C + c) / 8
+// at slot (r C + c) % 8 ^ s(r), C = chunks of a row. The swizzles s make the
+// copies (a row's chunks) and the fragment loads (below) free of bank conflicts:
+// K: eight lanes read four chunks of rows r, r + 1; V: two chunks (of pairs
+// of lanes) of rows i, 4 + i, 8 + i, 12 + i.
+template <int D, bool kS8, bool kFull>
+struct Ring {
+    static constexpr uint32_t kTiles = kS8 || D == 64 ? 2 : 1;     // tiles of a step
+    static constexpr uint32_t kChunk = 16 * kTiles;                // keys of a step
+    static constexpr uint32_t kSteps = kS8 ? 2 : 3;                // steps in the ring
+    static constexpr uint32_t kC = D * (kS8 ? 1 : 2) / 16;         // chunks of a row
+    static constexpr uint32_t kOperand = 16 * kC * 16;             // bytes of a tile of K or V
+    static constexpr uint32_t kStep = kTiles * 2 * kOperand;       // K tiles, then V tiles
+    static constexpr uint32_t kBytes = kSteps * (kStep + (kS8 ? 16 : 0));  // of a warp
+
+    static __device__ __forceinline__ uint32_t place_k(uint32_t row, uint32_t chunk) {
+        const uint32_t x = row * kC + chunk;
+        return kC == 4 ? x * 16 : (x ^ ((row & 1) << 2)) * 16;
+    }
+    static __device__ __forceinline__ uint32_t place_v(uint32_t row, uint32_t chunk) {
+        const uint32_t x = row * kC + chunk, q = (row >> 2) & 3;
+        return (x ^ (kC == 16 ? (q & 1) | ((q >> 1) << 2) : q << 1)) * 16;
     }
 
-    // The pages of the chunk at key0 (codes), fetched ahead of their use.
+    const RowsParams& p;
+    uint32_t base, scales;  // shared memory of this warp
+    uint32_t seq, kv_head, len, lane;
+    const uint32_t d;
+    int32_t page_next[kTiles];  // pages of the step to be issued next (codes), fetched a step ahead
+
+    __device__ Ring(const RowsParams& p, uint8_t* smem, uint32_t seq, uint32_t kv_head, uint32_t len)
+        : p(p), seq(seq), kv_head(kv_head), len(len), lane(threadIdx.x & 31), d(kFull ? D : p.head_dim) {
+        const uint32_t warp = threadIdx.x >> 5;
+        base = smem_addr(smem) + warp * (kSteps * kStep);
+        scales = smem_addr(smem) + kWarps * kSteps * kStep + warp * (kSteps * 16);
+    }
+
     __device__ __forceinline__ void fetch_pages(uint32_t key0) {
         if constexpr (kS8) {
 #pragma unroll
-            for (int b = 0; b < kTiles; ++b) {
+            for (uint32_t b = 0; b < kTiles; ++b) {
                 const uint32_t key = key0 + 16 * b;
                 page_next[b] =
                     key < len ? p.page_table[(uint64_t)seq * p.table_stride + (key >> p.page_shift)] : -1;
@@ -127,101 +161,72 @@ struct Source {
         }
     }
 
-    __device__ __forceinline__ uint64_t tile_of(int32_t page, uint32_t key) const {
-        const uint64_t unit = (uint64_t)(uint32_t)page * p.kv_heads + kv_head;
-        return ((unit << p.page_shift) + (key & ((1u << p.page_shift) - 1))) * d;
-    }
-
-    __device__ __forceinline__ void load_k(uint32_t key0) {
-        if constexpr (kS8) {
+    // Copies of the step's keys, one group whether or not there is anything to copy.
+    __device__ __forceinline__ void issue(uint32_t key0, uint32_t step, bool live) {
+        if (live) {
+            const uint32_t to = base + step * kStep, chunks = d * (kS8 ? 1 : 2) / 16;
 #pragma unroll
-            for (int b = 0; b < kTiles; ++b) {
+            for (uint32_t b = 0; b < kTiles; ++b) {
                 const uint32_t key = key0 + 16 * b;
-                int32_t page = page_next[b];
-                if (page < 0 || (uint32_t)page >= p.pages) {
-                    if (key < len && threadIdx.x % 32 == 0) atomicExch(p.err, 3);
-                    page = -1;
+                const uint8_t *k, *v;
+                uint64_t k_row, v_row;  // bytes from row to row
+                bool good = true;
+                if constexpr (kS8) {
+                    const int32_t page = page_next[b];
+                    good = page >= 0 && (uint32_t)page < p.pages;
+                    if (!good && key < len && lane == 0) atomicExch(p.err, 3);
+                    const uint64_t unit = (uint64_t)(uint32_t)(good ? page : 0) * p.kv_heads + kv_head;
+                    const uint64_t at = ((unit << p.page_shift) + (key & ((1u << p.page_shift) - 1))) * d;
+                    k = static_cast<const uint8_t*>(p.k) + at, v = static_cast<const uint8_t*>(p.v) + at;
+                    k_row = v_row = d;
+                    // scales; -1 and 0: no page of the cache, its keys are left out
+                    const uint32_t slot = scales + step * 16 + (lane & 1) * 4 * kTiles + 4 * b;
+                    if (lane < 2) {
+                        if (good) copy4(slot, (lane ? p.v_scales : p.k_scales) + unit);
+                        else asm volatile("st.shared.f32 [%0], %1;" ::"r"(slot), "f"(lane ? 0.0f : -1.0f) : "memory");
+                    }
+                } else {
+                    k = static_cast<const uint8_t*>(p.k) + 2 * (seq * p.k_batch + (uint64_t)kv_head * d + key * p.k_stride);
+                    v = static_cast<const uint8_t*>(p.v) + 2 * (seq * p.v_batch + (uint64_t)kv_head * d + key * p.v_stride);
+                    k_row = 2 * p.k_stride, v_row = 2 * p.v_stride;
                 }
-                page_k[b] = page;
-                sk[b] = sv[b] = 0.0f;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < kK; ++i) k[b][h][i] = make_uint4(0, 0, 0, 0);
-                if (page < 0) continue;
-                const uint64_t unit = (uint64_t)(uint32_t)page * p.kv_heads + kv_head;
-                sk[b] = p.k_scales[unit], sv[b] = p.v_scales[unit];
-                const int8_t* from = static_cast<const int8_t*>(p.k) + tile_of(page, key) + at_k;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < kK; ++i)
-                        if (kFull || 64 * i + 16 * t < d)
-                            k[b][h][i] = *reinterpret_cast<const uint4*>(from + 2 * h * d + 64 * i);
+                for (uint32_t i = 0; i < kC / 2; ++i) {
+                    const uint32_t x = i * 32 + lane, row = x / kC, chunk = x % kC;
+                    const uint32_t to_k = to + b * kOperand + place_k(row, chunk);
+                    const uint32_t to_v = to + (kTiles + b) * kOperand + place_v(row, chunk);
+                    if constexpr (kS8 && kFull) {  // the tile's 16 rows are consecutive
+                        copy16(to_k, k + x * 16, good);
+                        copy16(to_v, v + x * 16, good);
+                    } else {
+                        // past the end zeros: there may be no memory, or NaN
+                        const bool read = good && (kFull || chunk < chunks) && (kS8 || key + row < len);
+                        copy16(to_k, read ? k + row * k_row + chunk * 16 : p.k, read);
+                        copy16(to_v, read ? v + row * v_row + chunk * 16 : p.v, read);
+                    }
+                }
             }
-        } else {
-            // rows past the end are not read: they may be no memory, or hold NaN
-            const uint16_t* from = static_cast<const uint16_t*>(p.k) + at_k + key0 * p.k_stride;
-            const uint32_t key = key0 + 4 * (g >> 1) + (g & 1);
-#pragma unroll
-            for (int b = 0; b < kTiles; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < kK; ++i)
-                        k[b][h][i] = (kFull || 32 * i + 8 * t < d) && key + 16 * b + 2 * h < len
-                                         ? *reinterpret_cast<const uint4*>(from + (16 * b + 2 * h) * p.k_stride + 32 * i)
-                                         : make_uint4(0, 0, 0, 0);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
-    __device__ __forceinline__ void load_v(uint32_t key0) {
-        if constexpr (kS8) {
-#pragma unroll
-            for (int b = 0; b < kTiles; ++b) {
-                page_v[b] = page_k[b];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kV; ++j) v[b][i][j] = 0;
-                if (page_v[b] < 0 || !(kFull || D / 8 * g < d)) continue;
-                const int8_t* from = static_cast<const int8_t*>(p.v) + tile_of(page_v[b], key0 + 16 * b) + at_v;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (D == 128) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(from + i * d);
-                        v[b][i][0] = x.x, v[b][i][1] = x.y, v[b][i][2] = x.z, v[b][i][3] = x.w;
-                    } else {
-                        const uint2 x = *reinterpret_cast<const uint2*>(from + i * d);
-                        v[b][i][0] = x.x, v[b][i][1] = x.y;
-                    }
-                }
-            }
-        } else {
-            const uint16_t* from = static_cast<const uint16_t*>(p.v) + at_v + key0 * p.v_stride;
-#pragma unroll
-            for (int b = 0; b < kTiles; ++b)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < kV; j += 4) {
-                        const uint4 x = (kFull || D / 8 * g + 2 * j < d) && key0 + 16 * b + 4 * t + i < len
-                                            ? *reinterpret_cast<const uint4*>(from + (16 * b + i) * p.v_stride + 2 * j)
-                                            : make_uint4(0, 0, 0, 0);
-                        v[b][i][j] = x.x, v[b][i][j + 1] = x.y, v[b][i][j + 2] = x.z, v[b][i][j + 3] = x.w;
-                    }
-        }
+    // The oldest of kSteps - 1 groups has landed, for all lanes; all have left the step before.
+    __device__ __forceinline__ void wait() const {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSteps - 2) : "memory");
+        __syncwarp();
     }
 };
 
 // kBF16: type of the second product's operands (false for codes).
 template <int D, int NT, bool kS8, bool kBF16, bool kFull>
 __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsParams p) {
-    using Keys = Source<D, kS8, kFull>;
+    using Keys = Ring<D, kS8, kFull>;
     constexpr int kSteps = D / 16, kTiles = Keys::kTiles;
     constexpr uint32_t kChunk = Keys::kChunk;
     constexpr int R = 8 * NT;
-    __shared__ float s_o[kWarps][R][D + 4];
+    extern __shared__ __align__(128) uint8_t smem[];
+    // the rings' memory takes the warps' results at the end
+    auto s_o = reinterpret_cast<float (*)[R][D + 4]>(smem);
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
     __shared__ float c_m[kWarps * R], c_l[kWarps * R];  // of the block's rows, for the cluster
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     const uint32_t chunks = (len + kChunk - 1) / kChunk;
     const uint32_t per_split = (chunks + p.splits - 1) / p.splits;
     const uint32_t first = blockIdx.z * per_split;
-    Keys f(p, where.seq, kv_head, len, lane);
+    Keys f(p, smem, where.seq, kv_head, len);
     uint32_t c = first + key_warp;
     f.fetch_pages(c * kChunk);
 
@@ -303,56 +308,72 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.0f;
-        m[n][0] = m[n][1] = -INFINITY;
+        m[n][0] = m[n][1] = kLowest;
         l[n][0] = l[n][1] = 0.0f;
     }
 
-    // Two loads are in flight at any time: K of the next chunk from the first product
-    // on, V of the next chunk from the second on, into the registers just used.
-    if (c < last) {
-        f.load_k(c * kChunk);
-        f.load_v(c * kChunk);
-        f.fetch_pages((c + key_warps) * kChunk);
+    // fragment addresses: K rows g and g + 8 of S^T (keys 4 (g / 2) + g % 2 and the
+    // second next), V keys 4t .. 4t + 3
+    const uint32_t kr = 4 * (g >> 1) + (g & 1);
+    uint32_t step = 0, step_in = 0;
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < Keys::kSteps; ++i) {
+        const uint32_t ci = c + i * key_warps;
+        f.issue(ci * kChunk, step_in++, ci < last);
+        f.fetch_pages((ci + key_warps) * kChunk);
     }
     for (; c < last; c += key_warps) {
-        const uint32_t key0 = c * kChunk, next = (c + key_warps) * kChunk;
-        const bool more = c + key_warps < last;
+        const uint32_t key0 = c * kChunk;
+        f.wait();
+        {
+            const uint32_t ci = c + (Keys::kSteps - 1) * key_warps;
+            f.issue(ci * kChunk, step_in, ci < last);
+            f.fetch_pages((ci + key_warps) * kChunk);
+            step_in = step_in + 1 == Keys::kSteps ? 0 : step_in + 1;
+        }
+        const uint32_t from = f.base + step * Keys::kStep;
+        float sk[kTiles], sv[kTiles], sv_top = 0.0f;
+        bool any_dead = false;
+#pragma unroll
+        for (int b = 0; b < kTiles; ++b) {
+            sk[b] = sv[b] = 1.0f;
+            if constexpr (kS8) {
+                const uint32_t at = f.scales + step * 16 + 4 * b;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk[b]) : "r"(at) : "memory");
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sv[b]) : "r"(at + 4 * kTiles) : "memory");
+                any_dead |= sk[b] < 0.0f;
+            }
+            sv_top = fmaxf(sv_top, sv[b]);
+        }
+        step = step + 1 == Keys::kSteps ? 0 : step + 1;
         float sc[kTiles][NT][4];
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
+            const uint32_t k = from + b * Keys::kOperand;
 #pragma unroll
             for (int n = 0; n < NT; ++n) sc[b][n][0] = sc[b][n][1] = sc[b][n][2] = sc[b][n][3] = 0.0f;
-            if constexpr (kS8) {
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j) {
-                    const uint32_t x = word(f.k[b][0][j / 4], j % 4) ^ 0x80808080u;
-                    const uint32_t y = word(f.k[b][1][j / 4], j % 4) ^ 0x80808080u;
-                    const uint32_t a0 = codes_lo(x), a1 = codes_lo(y), a2 = codes_hi(x), a3 = codes_hi(y);
+            for (int i = 0; i < (int)Keys::kC / 4; ++i) {
+                const uint4 x4 = read16(k + Keys::place_k(kr, 4 * i + t)), y4 = read16(k + Keys::place_k(kr + 2, 4 * i + t));
+                if constexpr (kS8) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_16816<false>(sc[b][n], a0, a1, a2, a3, qf[n][j][0], qf[n][j][1]);
-                }
-            } else {
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t x = word(x4, j) ^ 0x80808080u, y = word(y4, j) ^ 0x80808080u;
+                        const uint32_t a0 = codes_lo(x), a1 = codes_lo(y), a2 = codes_hi(x), a3 = codes_hi(y);
 #pragma unroll
-                for (int j = 0; j < kSteps; ++j) {
-                    const uint4 &x = f.k[b][0][j / 2], &y = f.k[b][1][j / 2];
-                    const int i = 2 * (j % 2);
+                        for (int n = 0; n < NT; ++n)
+                            mma_16816<false>(sc[b][n], a0, a1, a2, a3, qf[n][4 * i + j][0], qf[n][4 * i + j][1]);
+                    }
+                } else {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        mma_16816<kBF16>(sc[b][n], word(x, i), word(y, i), word(x, i + 1), word(y, i + 1),
-                                         qf[n][j][0], qf[n][j][1]);
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma_16816<kBF16>(sc[b][n], word(x4, 2 * j), word(y4, 2 * j), word(x4, 2 * j + 1),
+                                             word(y4, 2 * j + 1), qf[n][2 * i + j][0], qf[n][2 * i + j][1]);
                 }
             }
         }
-        float sk[kTiles], sv[kTiles], sv_top = 0.0f;
-        bool dead[kTiles], any_dead = false;
-#pragma unroll
-        for (int b = 0; b < kTiles; ++b) {
-            sk[b] = kS8 ? f.sk[b] : 1.0f, sv[b] = kS8 ? f.sv[b] : 1.0f;
-            sv_top = fmaxf(sv_top, sv[b]);
-            dead[b] = kS8 && f.page_k[b] < 0;
-            any_dead |= dead[b];
-        }
-        if (more) f.load_k(next);
         // scores in units of log2, the keys out of reach at -inf
         bool raise = false;
 #pragma unroll
@@ -369,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (dead[b] || key + 16 * b + (e >= 2 ? 2 : 0) >= reach[n][e & 1]) sc[b][n][e] = -INFINITY;
+                        if (sk[b] < 0.0f || key + 16 * b + (e >= 2 ? 2 : 0) >= reach[n][e & 1]) sc[b][n][e] = -INFINITY;
         }
         float top[NT][2];
 #pragma unroll
@@ -395,7 +416,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
                     for (int k = 4; k < 32; k *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, k));
                     x = fmaxf(x, m[n][e]);
-                    const float down = x == -INFINITY ? 1.0f : ex2_approx(m[n][e] - x);
+                    const float down = ex2_approx(m[n][e] - x);
                     m[n][e] = x;
                     l[n][e] *= down;
 #pragma unroll
@@ -410,10 +431,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             for (int n = 0; n < NT; ++n) {
                 float e4[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mm = m[n][e & 1];
-                    e4[e] = ex2_approx(sc[b][n][e] - (mm == -INFINITY ? 0.0f : mm));
-                }
+                for (int e = 0; e < 4; ++e) e4[e] = ex2_approx(sc[b][n][e] - m[n][e & 1]);
                 l[n][0] += e4[0] + e4[2];
                 l[n][1] += e4[1] + e4[3];
                 pf[b][n][0] = transpose8x8(pack2<kBF16>(e4[0] * weight, e4[1] * weight));
@@ -422,10 +440,25 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         }
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
-            const auto& v = f.v[b];
-            if constexpr (kS8) {
+            const uint32_t from_v = from + (kTiles + b) * Keys::kOperand;
+            constexpr int kV = D * (kS8 ? 1 : 2) / 32;  // words of a lane's part of a V row
+            uint32_t v[4][kV];
 #pragma unroll
-                for (int i = 0; i < f.kV; ++i) {
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (kV == 2) {
+                    const uint2 x = read8(from_v + Keys::place_v(4 * t + i, g >> 1) + 8 * (g & 1));
+                    v[i][0] = x.x, v[i][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kV; j += 4) {
+                        const uint4 x = read16(from_v + Keys::place_v(4 * t + i, kV / 4 * g + j / 4));
+                        v[i][j] = x.x, v[i][j + 1] = x.y, v[i][j + 2] = x.z, v[i][j + 3] = x.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kV; ++i) {
+                if constexpr (kS8) {
                     const uint32_t x0 = v[0][i] ^ 0x80808080u, x1 = v[1][i] ^ 0x80808080u;
                     const uint32_t x2 = v[2][i] ^ 0x80808080u, x3 = v[3][i] ^ 0x80808080u;
                     const uint32_t l01 = prmt(x0, x1, 0x5140), h01 = prmt(x0, x1, 0x7362);
@@ -437,10 +470,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                         mma_16816<false>(o[2 * i + 1][n], codes_lo(h01), codes_hi(h01), codes_lo(h23), codes_hi(h23),
                                          pf[b][n][0], pf[b][n][1]);
                     }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < f.kV; ++i) {
+                } else {
                     const uint32_t a0 = prmt(v[0][i], v[1][i], 0x5410), a1 = prmt(v[0][i], v[1][i], 0x7632);
                     const uint32_t a2 = prmt(v[2][i], v[3][i], 0x5410), a3 = prmt(v[2][i], v[3][i], 0x7632);
 #pragma unroll
@@ -448,11 +478,10 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                 }
             }
         }
-        if (more) {
-            f.load_v(next);
-            f.fetch_pages(next + key_warps * kChunk);
-        }
     }
+    // the copies still under way are empty or will not be read, but they write to the rings
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
 
     // this warp's result: sums over the lanes that share a column, O in true units
     const float unit = kS8 ? ref * (1.0f / 128.0f) : kBF16 ? 1.0f : 1.0f / 128.0f;
@@ -472,16 +501,17 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         }
     __syncthreads();
 
+    // the join may be launched; it waits for this grid's end before it reads
+    if (p.splits > 1 && !p.clusters) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // merge the key warps of each row tile: a thread takes two dims of a row
     for (uint32_t i = threadIdx.x; i < tile_rows * (D / 2); i += kThreads) {
         const uint32_t r = i / (D / 2), dim = 2 * (i - r * (D / 2));
         const uint32_t w0 = r / R * key_warps, col = r % R, row = where.tile * tile_rows + r;
         if (row >= rows || dim >= d) continue;
-        float top = -INFINITY;
+        float top = kLowest;
         for (uint32_t k = 0; k < key_warps; ++k) top = fmaxf(top, s_m[w0 + k][col]);
         float sum = 0.0f, x[2] = {0.0f, 0.0f};
         for (uint32_t k = 0; k < key_warps; ++k) {
-            if (s_m[w0 + k][col] == -INFINITY) continue;
             const float a = ex2_approx(s_m[w0 + k][col] - top);
             sum += a * s_l[w0 + k][col];
             const float2 b = *reinterpret_cast<const float2*>(&s_o[w0 + k][col][dim]);
@@ -508,13 +538,11 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         const uint32_t r = i / (D / 2), dim = 2 * (i - r * (D / 2));
         const uint32_t w0 = r / R * key_warps, col = r % R, row = where.tile * tile_rows + r;
         if (row >= rows || dim >= d) continue;
-        float top = -INFINITY;
+        float top = kLowest;
         for (uint32_t k = 0; k < p.splits; ++k) top = fmaxf(top, cluster_load(cluster_place(&c_m[r], k)));
         float sum = 0.0f, x[2] = {0.0f, 0.0f};
         for (uint32_t k = 0; k < p.splits; ++k) {
-            const float mk = cluster_load(cluster_place(&c_m[r], k));
-            if (mk == -INFINITY) continue;
-            const float a = ex2_approx(mk - top);
+            const float a = ex2_approx(cluster_load(cluster_place(&c_m[r], k)) - top);
             sum += a * cluster_load(cluster_place(&c_l[r], k));
             const float2 b = cluster_load2(cluster_place(&s_o[w0][col][dim], k));
             x[0] += a * b.x;
@@ -527,40 +555,61 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     cluster_sync();  // no block leaves while another reads its shared memory
 }
 
-// Joins the splits of each row: a warp to a row.
+// Joins the splits of a row: each warp every fourth split, four dims to a lane, then
+// the warps' sums. Launched while the rows kernel still runs; waits for its end.
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const RowsParams p) {
-    const uint32_t lane = threadIdx.x & 31;
-    const uint64_t row = (uint64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+    __shared__ float s_f[kMaxSplits];
+    __shared__ float4 s_x[kWarps][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t row = blockIdx.x;
     const uint32_t heads = p.kv_heads * p.group;
     const uint64_t token = row / heads;
-    const uint64_t tokens = p.query_begin ? p.queries : (uint64_t)p.sequences * p.queries;
-    if (token >= tokens) return;
+    const uint32_t head = (uint32_t)(row - token * heads);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // rows of no sequence stay as they were
     if (p.query_begin && ((int64_t)token < p.query_begin[0] || (int64_t)token >= p.query_begin[p.sequences])) return;
-    const uint32_t head = (uint32_t)(row - token * heads);
-    const float2* ml = p.part_ml + row * p.splits;
-    float top = -INFINITY;
-    for (uint32_t k = lane; k < p.splits; k += 32) top = fmaxf(top, ml[k].x);
+    float top = kLowest, sum = 0.0f;
+    float2 ml[kMaxSplits / 32];
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSplits / 32; ++i) {
+        const uint32_t k = 32 * i + lane;
+        ml[i] = k < p.splits ? p.part_ml[row * p.splits + k] : make_float2(kLowest, 0.0f);
+        top = fmaxf(top, ml[i].x);
+    }
     top = warp_max(top);
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSplits / 32; ++i) {
+        const float f = ml[i].y > 0.0f ? ex2_approx(ml[i].x - top) : 0.0f;
+        sum += f * ml[i].y;
+        if (warp == 0) s_f[32 * i + lane] = f;
+    }
+    sum = warp_sum(sum);
+    __syncthreads();
     const uint32_t dim = 4 * lane;
-    for (uint32_t k = 0; k < p.splits; ++k) {
-        const float2 a = ml[k];
-        if (!(a.y > 0.0f)) continue;
-        const float f = ex2_approx(a.x - top);
-        sum += f * a.y;
-        if (dim < p.head_dim) {
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (dim < p.head_dim) {
+#pragma unroll 8
+        for (uint32_t k = warp; k < p.splits; k += kWarps) {
+            const float f = s_f[k];
+            if (f == 0.0f) continue;  // no key of the split in reach: nothing was written
             const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + k) * p.head_dim + dim);
-            x[0] += f * o.x, x[1] += f * o.y, x[2] += f * o.z, x[3] += f * o.w;
+            x.x += f * o.x, x.y += f * o.y, x.z += f * o.z, x.w += f * o.w;
         }
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    s_x[warp][lane] = x;
+    __syncthreads();
+    if (warp || dim >= p.head_dim) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] *= inv;
+    for (uint32_t w = 1; w < kWarps; ++w) {
+        const float4 y = s_x[w][lane];
+        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
     const uint64_t batch = p.query_begin ? 0 : token / p.queries;
-    const uint64_t at = batch * p.out_batch + (token - batch * p.queries) * p.out_stride + (uint64_t)head * p.head_dim;
-    const uint64_t flat = token * p.out_stride + (uint64_t)head * p.head_dim;
-    if (dim < p.head_dim) store_out(p, (p.query_begin ? flat : at) + dim, x, 4);
+    const uint64_t at = p.query_begin ? token * p.out_stride
+                                      : batch * p.out_batch + (token - batch * p.queries) * p.out_stride;
+    store_out(p, at + (uint64_t)head * p.head_dim + dim, y, 4);
 }
 
 template <int D, int NT, bool kS8, bool kBF16, bool kFull>
@@ -568,13 +617,26 @@ int start(const RowsParams& p, uint32_t slots, cudaStream_t st) {
     cudaLaunchAttribute cluster[1];
     cluster[0].id = cudaLaunchAttributeClusterDimension;
     cluster[0].val.clusterDim.x = 1, cluster[0].val.clusterDim.y = 1, cluster[0].val.clusterDim.z = p.splits;
+    constexpr uint32_t kSmem = std::max<uint32_t>(kWarps * Ring<D, kS8, kFull>::kBytes, kWarps * 8 * NT * (D + 4) * 4);
+    auto kernel = attention_rows_kernel<D, NT, kS8, kBF16, kFull>;
+    static std::atomic<uint64_t> configured;  // one bit per device ordinal
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!configured_on(configured, dev)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess ||
+            cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 (int)cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+            return set_error(DAV2CUDA_LAUNCH_FAILED, "attention: cannot set shared memory size");
+        mark_configured(configured, dev);
+    }
     cudaLaunchConfig_t config{};
+    config.dynamicSmemBytes = kSmem;
     config.gridDim = dim3(slots, p.kv_heads, p.splits);
     config.blockDim = dim3(kThreads);
     config.stream = st;
     config.attrs = cluster;
     config.numAttrs = p.clusters ? 1 : 0;
-    cudaLaunchKernelEx(&config, attention_rows_kernel<D, NT, kS8, kBF16, kFull>, p);
+    cudaLaunchKernelEx(&config, kernel, p);
     return check_launch("attention_rows");
 }
 
@@ -599,7 +661,16 @@ int launch_attention_rows(const RowsParams& p, uint32_t slots, uint32_t row_tile
 }
 
 int launch_attention_join(const RowsParams& p, uint64_t rows, cudaStream_t st) {
-    attention_join_kernel<<<(uint32_t)((rows + kWarps - 1) / kWarps), kThreads, 0, st>>>(p);
+    cudaLaunchAttribute early[1];
+    early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((uint32_t)rows);
+    config.blockDim = dim3(kThreads);
+    config.stream = st;
+    config.attrs = early;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, attention_join_kernel, p);
     return check_launch("attention_join");
 }
 

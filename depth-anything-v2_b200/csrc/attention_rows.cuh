@@ -6,6 +6,8 @@
 
 namespace dav2cuda {
 
+constexpr uint32_t kMaxSplits = 128;
+
 struct RowsParams {
     void* out;
     const void* q;

@@ -340,6 +340,7 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
+            if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             if (ok) ok = warp_wait(o_full, 0);
             tc_fence_after();
             if (ok) {
