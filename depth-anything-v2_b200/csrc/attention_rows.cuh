@@ -77,12 +77,9 @@ struct RowTile {
 
 __device__ __forceinline__ bool find_row_tile(RowTile& f, const RowsParams& p, uint32_t block, uint32_t tile_rows) {
     if (p.query_begin) {
-        uint32_t s = 0;
-        for (uint32_t high = p.sequences; high - s > 1;) {
-            const uint32_t mid = (s + high) / 2;
-            if ((uint64_t)(uint32_t)p.query_begin[mid] * p.group / tile_rows + mid <= block) s = mid;
-            else high = mid;
-        }
+        const uint32_t s = warp_last_at_most(p.sequences, block, [&](uint32_t i) {
+            return (uint64_t)(uint32_t)p.query_begin[i] * p.group / tile_rows + i;
+        });
         const int32_t b = p.query_begin[s], e = p.query_begin[s + 1];
         if (b < 0 || e < b || (uint32_t)e > p.queries) {
             if (threadIdx.x == 0) atomicExch(p.err, 3);

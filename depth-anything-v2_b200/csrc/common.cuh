@@ -293,6 +293,23 @@ __device__ __forceinline__ float warp_min(float v) {
     return v;
 }
 
+// The last of n indices (n >= 1) whose value first(i), rising with i, is at most
+// `block`; 0 if none is. A warp looks at 32 places at a time, so that a thousand
+// entries of a device array cost two loads in a row.
+template <typename F>
+__device__ __forceinline__ uint32_t warp_last_at_most(uint32_t n, uint64_t block, F first) {
+    const uint32_t lane = threadIdx.x & 31;
+    uint32_t low = 0;
+    while (n > 1) {
+        const uint32_t step = (n + 31) / 32, at = lane * step;
+        const uint32_t below = __popc(__ballot_sync(0xffffffffu, at < n && first(low + at) <= block));
+        const uint32_t skip = (below ? below - 1 : 0) * step;
+        low += skip;
+        n = min(step, n - skip);
+    }
+    return low;
+}
+
 // code = rint(clamp(v, -127, 127)) as a byte (ties to even, as the
 // reference's CPU packers: std::nearbyint).
 __device__ __forceinline__ uint32_t q8(float v) {

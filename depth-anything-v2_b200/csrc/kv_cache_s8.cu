@@ -59,12 +59,9 @@ __global__ void __launch_bounds__(kThreads) kv_cache_append_kernel(const AppendP
     const uint32_t which = blockIdx.z, head = blockIdx.y;
     const uint32_t page_tokens = 1u << p.page_shift;
     // the last sequence whose blocks begin at or before this one
-    uint32_t s = 0;
-    for (uint32_t high = p.sequences; high - s > 1;) {
-        const uint32_t mid = (s + high) / 2;
-        if (((uint32_t)p.begin[mid] >> p.page_shift) + 2 * mid <= blockIdx.x) s = mid;
-        else high = mid;
-    }
+    const uint32_t s = warp_last_at_most(p.sequences, blockIdx.x, [&](uint32_t i) {
+        return (uint64_t)((uint32_t)p.begin[i] >> p.page_shift) + 2 * i;
+    });
     const int64_t begin = p.begin[s], end = p.begin[s + 1], cached = p.cached[s];
     const int64_t j = (int64_t)blockIdx.x - ((begin >> p.page_shift) + 2 * (int64_t)s);
     if (j < 0) return;  // rows before the first sequence
