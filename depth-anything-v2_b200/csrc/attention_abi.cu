@@ -39,7 +39,18 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_lengt
     const uint64_t live = std::max<uint64_t>(1, sequences * ((rows + tile - 1) / tile)) * kv_heads;
     n.clusters = false;
     if (!n.row_warps) {
-        n.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(kSms / live, max_length / 256));
+        // the split count that ends first: rounds of units over the SMs, each a number of
+        // 128-key blocks (about 2 us) and about four more to begin and end; the parts are
+        // written and read at about 5 TB/s, and their join is a launch
+        const uint64_t blocks = (max_length + 127ull) / 128;
+        const uint64_t part = rows * sequences * kv_heads * (head_dim * 8ull + 16);
+        uint64_t best = ~0ull;
+        n.splits = 1;
+        for (uint64_t s = 1; s <= 32 && s * 4 <= std::max<uint64_t>(blocks, 4); ++s) {
+            const uint64_t cost = (live * s + kSms - 1) / kSms * ((blocks + s - 1) / s + 4) +
+                                  (s > 1 ? 3 + s * part / 10000000 : 0);
+            if (cost < best) best = cost, n.splits = (uint32_t)s;
+        }
         return n;
     }
     // The rows kernel. What fits the device at once is filled by one wave of equal

@@ -1,21 +1,29 @@
 // Attention of many query rows on tcgen05 tensor cores, for the two sources of
 // keys and values of attention_rows.cu (16-bit rows, pages of int8 codes).
 //
-// A block takes two tiles of 128 rows (query x head of the group that shares a key
-// head) and walks the keys in blocks of 128:
+// A unit of work is two tiles of 128 rows (query x head of the group that shares a key
+// head) against the keys in blocks of 128:
 //   S_t = Q_t K^T (128 x 128, f32 in tensor memory), P_t = 2^(S_t - m) in 16 bits,
 //   O_t += P_t V (128 x D, f32 in tensor memory), l_t += sum P_t
 // One thread owns one row: it loads its 128 scores, takes the maximum, exponentiates
 // and writes P into tensor memory, from where the second product reads it as its A
 // operand, so that P never passes through shared memory. m follows the row's maximum
 // only when that exceeds it by 8 (log2 units), and then the thread rescales its row
-// of O; S_t's barrier tells that the previous P V is done, since it was issued before.
-// While one tile's softmax runs, the tensor cores work on the other tile.
+// of O. While one tile's softmax runs, the tensor cores work on the other tile; at
+// D = 64 also S of the next block, as P has columns of its own.
 //
-//   warps 0-3, 4-7   softmax of tile 0, 1 (and, first, their rows of Q to shared memory)
-//   warp 8           products: P_0 V_j, S_0 of j + 1, P_1 V_j, S_1 of j + 1
-//   warp 9           16-bit rows: TMA of K_j, V_j into a ring of 128-key tiles
-//   warps 9-11       codes: int8 from the pages into the same tiles as f16
+// One block runs on an SM at a time and takes over the units of blocks that have not
+// started yet, one after the other (cluster launch control), so that units of different
+// lengths spread evenly; its roles run ahead of one another across units: Q and the first
+// keys of the next unit are loaded, and its first S computed, while the softmax warps
+// still write the last unit's rows.
+//
+//   warps 0-3, 4-7   softmax of tile 0, 1
+//   16-bit rows:     warps 8, 9 products (D = 64: S, P V; D = 128: of tile 0, 1); warp 10 TMA of K_j, V_j into a
+//                    ring of 128-key tiles; warp 11 rows of Q (TMA where the heads of a
+//                    group divide 128, else copies)
+//   codes:           warp 8 products of both; warps 9-11 int8 from the pages to f16 in
+//                    the same ring, and rows of Q, scaled by a power of two into f16's range
 // The 128-byte-swizzled tiles are 64 dims wide; heads above 64 take two of them.
 //
 // Keys past the end: scores are replaced by -inf; the rows of V behind the last
@@ -38,26 +46,72 @@ constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kKeys = 128;        // keys of a block
 constexpr uint32_t kAtom = 128 * 128;  // bytes of 128 rows x 64 dims of 16 bits
 constexpr float kRaise = 8.0f;
-constexpr uint32_t kSoftmaxThreads = 256;
-constexpr uint32_t kConverters = 3;    // 12 warps in all: 168 registers a thread
-
+constexpr uint32_t kSoftmaxWarps = 8;
+constexpr uint32_t kConverters = 3;      // codes
+constexpr uint32_t kThreads = 12 * 32;   // 168 registers each
+// Warps that issue products: one for each tile, so that what one does between its
+// products is hidden by the other's. Codes need the second warp for conversion.
 template <int D, bool kS8>
+constexpr uint32_t kIssuers = kS8 ? 1 : 2;
+// At D = 128, where S waits for P, the two take turns: products that interleave bring the
+// tiles into step, so that both softmaxes and then both products wait (128 x 5477 keys:
+// 98 us, without turns 130 us). At D = 64, where S runs ahead, turns cost 7%.
+template <int D>
+constexpr bool kTurns = D == 128;
+
+constexpr float kLowest = -3.402823466e38f;
+// Of eight pairs of exponentials, how many leave the exponential unit alone. Measured with
+// 0, 1, 2, 3, 4 of 8: 8 x 1370 x 1370, 16 heads of 64, 148, 141, 138, 142, 152 us; 4 x 1370 x
+// 5477, 16 heads of 128, 233, 229, 237, 231, 268 us.
+constexpr int kEmulated = 2;
+
+template <int D>
 struct Layout {
     static constexpr uint32_t kOperand = D / 64 * kAtom;   // bytes of 128 rows
-    static constexpr uint32_t kStages = D == 64 ? 8 : 5;   // K or V tiles in flight
-    static constexpr uint32_t kThreads = kSoftmaxThreads + (kS8 ? 1 + kConverters : 2) * 32;
-    static constexpr uint32_t kSmem = (2 + kStages) * kOperand + 1024;
-    // S_0, S_1, then O_0, O_1; P shares S's columns
+    static constexpr uint32_t kQBufs = D == 64 ? 2 : 1;    // Q of this unit and the next
+    static constexpr uint32_t kStages = D == 64 ? 8 : 5;    // K or V tiles in flight
+    static constexpr uint32_t kBackSlots = 2 * kQBufs;     // codes: units whose row factors are kept
+    static constexpr uint32_t kBars = 512;                  // bytes of barriers
+    static constexpr uint32_t kSmem =
+        (2 * kQBufs + kStages) * kOperand + kBars + kBackSlots * 2 * kTileRows;
+    // Tensor memory columns: S_0, S_1, O_0, O_1, and at D = 64 P_0, P_1; at D = 128,
+    // where S and O fill it, P_t takes the first half of S_t.
+    static constexpr bool kAlias = D == 128;
     static constexpr uint32_t kO = 256;
+    static constexpr uint32_t kP = kAlias ? 0 : 384, kPStride = kAlias ? 128 : 64;
+};
+static_assert(Layout<128>::kSmem <= 232448 && Layout<64>::kSmem <= 232448, "shared memory above the per-block limit");
+
+struct TilesParams {
+    uint32_t q_box;  // Q by TMA: tokens of a 128-row box (0: by a warp)
+    uint32_t slots, full_units, full_tiles;  // full_*: dense batches
 };
 
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+// The products, from the low words of their descriptors (address and one stride);
+// the high word is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // 8-row stride, version 1, 128-byte swizzle
+constexpr uint32_t kDescK = 1u << 16;             // K-major: no leading stride
+constexpr uint32_t kDescV = (kAtom >> 4) << 16;   // MN-major: 64-dim groups one atom apart
+
+template <bool kAccumulate>
+__device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint32_t desc_a, uint32_t desc_b, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(desc_a), "r"(desc_b), "r"(idesc), "n"(kAccumulate ? 1 : 0), "n"(kDescHigh)
+        : "memory");
+}
+
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t desc_b, uint32_t idesc,
                                         uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %5};\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "r"(desc_b), "r"(idesc), "r"(accumulate), "n"(kDescHigh)
         : "memory");
 }
 
@@ -74,18 +128,56 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8
                  : "memory");
 }
 
+// The largest of three; NaN if one is.
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
-// MN-major operand (V: keys x dims, dims contiguous), 128-byte swizzle: 8-key
-// groups 1024 B apart, 64-dim groups one atom apart.
-__device__ __forceinline__ uint64_t desc_v(uint32_t saddr) {
-    return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kAtom >> 4) << 16) |
-           (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
-           (static_cast<uint64_t>(2) << 61);
+// 2^x of two values without the exponential unit, which the softmax would otherwise be
+// bound by (a quarter of the rate of a multiply-add): x = n + f with |f| <= 1/2, a
+// polynomial of degree 4 for 2^f (minimax in the relative error, 2.7e-6 as evaluated),
+// and n added to the exponent. x <= 127; below -126 the result is 2^-126.
+__device__ __forceinline__ void exp2_pair(float& x, float& y) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it leaves rint(x) in the low bits
+    x = fmaxf(x, -126.0f), y = fmaxf(y, -126.0f);
+    float rx, ry, fx, fy, px, py;
+    f2_add(rx, ry, x, y, kMagic, kMagic);
+    f2_add(fx, fy, rx, ry, -kMagic, -kMagic);
+    f2_fma(fx, fy, fx, fy, -1.0f, -1.0f, x, y);
+    f2_fma(px, py, fx, fy, 0.009570102207362652f, 0.009570102207362652f, 0.05591785907745361f, 0.05591785907745361f);
+    f2_fma(px, py, px, py, fx, fy, 0.240247443318367f, 0.240247443318367f);
+    f2_fma(px, py, px, py, fx, fy, 0.6931217908859253f, 0.6931217908859253f);
+    f2_fma(px, py, px, py, fx, fy, 0.9999992847442627f, 0.9999992847442627f);
+    // the magic number's own bits are shifted out
+    x = __int_as_float(__float_as_int(px) + (__float_as_int(rx) << 23));
+    y = __int_as_float(__float_as_int(py) + (__float_as_int(ry) << 23));
+}
+
+// A block's next unit, by taking over the place of a block that has not started:
+// the hardware writes its index, or that there is none, and completes 16 bytes on the barrier.
+__device__ __forceinline__ void request_unit(uint4* response, uint64_t* bar) {
+    asm volatile(
+        "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+            smem_addr(response)),
+        "r"(smem_addr(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ bool read_unit(const uint4* response, uint32_t& unit) {
+    uint32_t taken, x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t.reg .b32 y, z, w;\n\t"
+        "ld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, r;\n\t}"
+        : "=r"(taken), "=r"(x)
+        : "r"(smem_addr(response))
+        : "memory");
+    unit = x;
+    return taken != 0;
 }
 
 // Byte of (row, 8-dim chunk) in a swizzled operand.
@@ -93,40 +185,86 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t row, uint32_t chunk) {
     return (chunk >> 3) * kAtom + row * 128u + (((chunk & 7u) ^ (row & 7u)) << 4);
 }
 
+// One unit of work: 256 rows of a sequence and key head, and a split of its keys.
+struct Unit {
+    RowTile where;
+    uint32_t kv_head, split, len, row0, tiles, first, blocks;
+    bool any;
+};
+
+// Units are numbered row tile first, then key head, then split, so that blocks that run
+// together share K and V in L2. Dense batches: the full tiles of all sequences, then
+// their last ones, which are shorter.
+__device__ __forceinline__ Unit unit_at(const RowsParams& p, const TilesParams& n, uint32_t u) {
+    Unit w;
+    w.where = RowTile{};
+    if (p.query_begin) {
+        const uint32_t slot = u % n.slots, x = u / n.slots;
+        w.kv_head = x % p.kv_heads;
+        w.split = x / p.kv_heads;
+        w.any = find_row_tile(w.where, p, slot, 2 * kTileRows);
+    } else {
+        uint32_t x;
+        if (u < n.full_units) {
+            x = u / n.full_tiles;
+            w.where.tile = u - x * n.full_tiles;
+        } else {
+            x = u - n.full_units;
+            w.where.tile = n.full_tiles;
+        }
+        w.kv_head = x % p.kv_heads;
+        x /= p.kv_heads;
+        w.where.seq = x % p.sequences;
+        w.split = x / p.sequences;
+        w.where.q_count = p.queries;
+        w.where.rows = p.queries * p.group;
+        w.any = true;
+    }
+    w.blocks = 0;
+    if (!w.any) return w;
+    w.len = keys_of(p, w.where.seq);
+    w.row0 = w.where.tile * 2 * kTileRows;
+    w.tiles = w.where.rows - w.row0 > kTileRows ? 2u : 1u;
+    // the key blocks of this split, up to the last row's reach
+    const uint32_t reach = reach_of(p, w.where, w.len, min(w.where.rows, w.row0 + 2 * kTileRows) - 1);
+    const uint32_t all = (w.len + kKeys - 1) / kKeys, per_split = (all + p.splits - 1) / p.splits;
+    w.first = w.split * per_split;
+    const uint32_t last = min(min(all, w.first + per_split), (reach + kKeys - 1) / kKeys);
+    w.blocks = last > w.first ? last - w.first : 0;
+    return w;
+}
+
 template <int D, bool kS8, bool kBF16>
-__global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
-    attention_tiles_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                           const RowsParams p) {
-    using L = Layout<D, kS8>;
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                           const __grid_constant__ CUtensorMap tm_v, const RowsParams p, const TilesParams n) {
+    using L = Layout<D>;
     constexpr uint32_t kStages = L::kStages;
+    constexpr uint32_t kQBufs = L::kQBufs;
     extern __shared__ uint8_t smem[];
     uint8_t* sQ = smem;                        // [tile]
-    uint8_t* sKV = smem + 2 * L::kOperand;     // [stage]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kStages * L::kOperand);
-    uint64_t* full = bars;               // [stage]
+    uint8_t* sKV = smem + 2 * kQBufs * L::kOperand;  // [stage]
+    uint8_t* control = sKV + kStages * L::kOperand;
+    uint4* response = reinterpret_cast<uint4*>(control);  // [2]
+    uint64_t* full = reinterpret_cast<uint64_t*>(response + 2);  // [stage]
     uint64_t* empty = full + kStages;    // [stage]
-    uint64_t* q_full = empty + kStages;  // [tile]
-    uint64_t* s_full = q_full + 2;       // [tile]
-    uint64_t* p_full = s_full + 2;       // [tile]
-    uint64_t* o_full = p_full + 2;
-    uint64_t* drain = o_full + 1;
-    float* s_top = reinterpret_cast<float*>(drain + 1);            // [warp]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_top + 16);
+    uint64_t* s_full = empty + kStages;  // [tile]
+    uint64_t* s_free = s_full + 2;       // [tile]: S is in registers (P beside S)
+    uint64_t* p_full = s_free + 2;       // [tile]
+    uint64_t* pv_done = p_full + 2;      // [tile]
+    uint64_t* o_full = pv_done + 2;      // [tile]
+    uint64_t* q_full = o_full + 2;       // [buffer]
+    uint64_t* q_empty = q_full + 2;      // [buffer]
+    uint64_t* unit_full = q_empty + 2;   // [response]
+    uint64_t* unit_empty = unit_full + 2;  // [response]
+    uint64_t* turn = unit_empty + 2;     // [tile]
+    uint64_t* drain = turn + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* s_top = reinterpret_cast<float*>(tmem_slot + 4);        // codes: [slot] the largest V scale
+    int8_t* s_back = reinterpret_cast<int8_t*>(control + L::kBars);  // codes: [slot][row] powers of two of Q
+    static_assert(32 + 8 * (2 * kStages + 22) + 32 <= L::kBars, "barriers overflow their part");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-    RowTile where;
-    if (!find_row_tile(where, p, blockIdx.x, 2 * kTileRows)) return;
-    const uint32_t kv_head = blockIdx.y;
-    const uint32_t len = keys_of(p, where.seq);
-    const uint32_t row0 = where.tile * 2 * kTileRows;
-    const uint32_t tiles = where.rows - row0 > kTileRows ? 2u : 1u;
-    // the key blocks of this split, up to the last row's reach
-    const uint32_t reach_top = reach_of(p, where, len, min(where.rows, row0 + 2 * kTileRows) - 1);
-    const uint32_t all = (len + kKeys - 1) / kKeys, per_split = (all + p.splits - 1) / p.splits;
-    const uint32_t first = blockIdx.z * per_split;
-    const uint32_t last = min(min(all, first + per_split), (reach_top + kKeys - 1) / kKeys);
-    const uint32_t blocks = last > first ? last - first : 0;
 
     if ((smem_addr(smem) & 1023u) != 0) {  // the 128-byte swizzle needs 1 KB aligned tiles
         if (threadIdx.x == 0) atomicExch(p.err, 2);
@@ -135,122 +273,108 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < kStages; ++i) {
             mbar_init(&full[i], kS8 ? kConverters : 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], kIssuers<D, kS8>);
         }
         for (uint32_t t = 0; t < 2; ++t) {
-            mbar_init(&q_full[t], 4);
             mbar_init(&s_full[t], 1);
+            mbar_init(&s_free[t], 4);
             mbar_init(&p_full[t], 4);
+            mbar_init(&pv_done[t], 1);
+            mbar_init(&o_full[t], 1);
+            mbar_init(&turn[t], 1);
+            mbar_init(&q_full[t], kS8 ? kConverters : 1);
+            mbar_init(&q_empty[t], kIssuers<D, kS8>);
+            mbar_init(&unit_full[t], 1);
+            mbar_init(&unit_empty[t], kSoftmaxWarps + kIssuers<D, kS8> + (kS8 ? kConverters : 2));  // warps at work
         }
-        mbar_init(o_full, 1);
-        mbar_init(drain, 1);
+        mbar_init(&drain[0], 1);
+        mbar_init(&drain[1], 1);
         *abort_flag = 0;
         fence_barrier_init();
         if (!kS8) {
+            if (n.q_box) tma_prefetch_desc(&tm_q);
             tma_prefetch_desc(&tm_k);
             tma_prefetch_desc(&tm_v);
         }
     }
-    if (warp == 8) tmem_alloc(tmem_slot, 512);
-    float v_top = 1.0f;
-    if constexpr (kS8) {
-        // the largest V scale of the keys in reach
-        float top = 0.0f;
-        const uint32_t page_end = (min(len, last * kKeys) + (1u << p.page_shift) - 1) >> p.page_shift;
-        for (uint32_t i = ((first * kKeys) >> p.page_shift) + threadIdx.x; i < page_end; i += L::kThreads) {
-            const int32_t page = p.page_table[(uint64_t)where.seq * p.table_stride + i];
-            if (page >= 0 && (uint32_t)page < p.pages)
-                top = fmaxf(top, p.v_scales[(uint64_t)page * p.kv_heads + kv_head]);
-        }
-        top = warp_max(top);
-        if (lane == 0) s_top[warp] = top;
-    }
+    if (warp == kSoftmaxWarps) tmem_alloc(tmem_slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    if constexpr (kS8) {
-        float top = 1e-30f;
-        for (uint32_t i = 0; i < L::kThreads / 32; ++i) top = fmaxf(top, s_top[i]);
-        v_top = top;
-    }
     bool mma_issued = false;
+    // a warp's lanes leave a wait together: the collective accesses below never diverge
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity & 1u, abort_flag, p.err));
+    };
 
-    if (warp < 8) {
+    // The unit after the `iter`-th one of this block; false: there is none (or a timeout).
+    auto next_unit = [&](uint32_t iter, uint32_t& u) -> bool {
+        const uint32_t slot = iter & 1u;
+        if (!warp_wait(&unit_full[slot], iter >> 1)) return false;
+        const bool more = read_unit(&response[slot], u);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&unit_empty[slot]);
+        return more;
+    };
+
+    if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax
         const uint32_t t = warp >> 2, quarter = warp & 3u;
-        const uint32_t r = quarter * 32u + lane;                      // row of the tile
-        const uint32_t row = row0 + t * kTileRows + r;                // row of the sequence
-        const uint32_t tS = tmem + t * 128u + ((quarter * 32u) << 16);
-        const uint32_t tO = tmem + L::kO + t * D + ((quarter * 32u) << 16);
-        const bool live = row < where.rows;
-        if (t < tiles && blocks) {
-            // this row of Q; a negative scale goes into its sign. For codes it is
-            // brought into f16's range by a power of two.
-            const uint16_t* q = static_cast<const uint16_t*>(p.q) +
-                                (live ? row_at(p, where, kv_head, row, p.q_batch, p.q_stride) : 0);
-            uint4 x[D / 8];
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-                x[i] = live && 8 * i < p.head_dim ? *reinterpret_cast<const uint4*>(q + 8 * i) : make_uint4(0, 0, 0, 0);
-            const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;
-            float c = fabsf(p.scale_log2);
-            if constexpr (kS8) {
-                float most = 0.0f;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    const uint32_t w4[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 a = unpack2(w4[e], p.q_bf16);
-                        most = fmax3(most, fabsf(a.x), fabsf(a.y));
-                    }
+        const uint32_t r = quarter * 32u + lane;  // row of the tile
+        const uint32_t lanes = (quarter * 32u) << 16;
+        const uint32_t tS = tmem + t * 128u + lanes, tP = tmem + L::kP + t * L::kPStride + lanes;
+        const uint32_t tO = tmem + L::kO + t * D + lanes;
+        uint32_t done = 0;   // blocks of this tile so far
+        uint32_t outs = 0;   // units of this tile so far
+        uint32_t units = 0;  // units with keys so far
+        bool ok = true;
+        uint32_t u = blockIdx.x;
+        for (uint32_t iter = 0;; ++iter) {
+            if (iter && !next_unit(iter - 1, u)) break;
+            const Unit w = unit_at(p, n, u);
+            if (!w.any) continue;
+            const uint32_t row = w.row0 + t * kTileRows + r;  // row of the sequence
+            const bool live = row < w.where.rows;
+            if (!w.blocks) {  // no key in reach
+                if (t >= w.tiles || !live) continue;
+                if (p.splits > 1) {
+                    p.part_ml[part_at(p, w.where, w.kv_head, row, w.split)] = make_float2(-INFINITY, 0.0f);
+                } else {
+                    const uint64_t at = row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
+                    const float zero[2] = {0.0f, 0.0f};
+                    for (uint32_t i = 0; i < p.head_dim; i += 2) store_out(p, at + i, zero, 2);
                 }
-                int e = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
-                e = max(-120, min(120, e));
-                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-                c *= __uint_as_float((uint32_t)(127 - e) << 23);
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-                    uint32_t* w4 = reinterpret_cast<uint32_t*>(&x[i]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float2 a = unpack2(w4[k], p.q_bf16);
-                        w4[k] = pack2<false>(a.x * up, a.y * up);
-                    }
-                }
+                continue;
             }
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-                *reinterpret_cast<uint4*>(sQ + t * L::kOperand + chunk_at(r, i)) =
-                    make_uint4(x[i].x ^ sign, x[i].y ^ sign, x[i].z ^ sign, x[i].w ^ sign);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[t]);
-
-            const uint32_t reach = reach_of(p, where, len, row);
+            const uint32_t unit = units++;
+            if (t >= w.tiles) continue;
+            // a negative scale is in the first product's sign; above 0, so that the -inf of a masked key stays
+            float c = fmaxf(fabsf(p.scale_log2), 1e-35f), v_top = 1.0f;
+            if constexpr (kS8) {
+                if (!warp_wait(&q_full[unit % kQBufs], unit / kQBufs)) break;
+                c *= __uint_as_float((uint32_t)(127 - s_back[unit % L::kBackSlots * 2 * kTileRows + t * kTileRows + r]) << 23);
+                v_top = s_top[unit % L::kBackSlots];
+            }
+            const uint32_t reach = reach_of(p, w.where, w.len, row);
             const uint32_t low = __reduce_min_sync(0xffffffffu, live ? reach : 0xFFFFFFFFu);
-            auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-                return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err));
-            };
             // codes: lane i has the K scale (i < 8), lane 8 + i the V scale over the largest,
             // of the block's keys 16i .. 16i + 15; fetched a block ahead. -1: no such page
             auto scale_of = [&](uint32_t j) -> float {
-                const uint32_t key = (first + j) * kKeys + 16u * (lane & 7u);
-                if (lane >= 16 || key >= len) return 0.0f;
-                const int32_t page = p.page_table[(uint64_t)where.seq * p.table_stride + (key >> p.page_shift)];
+                const uint32_t key = (w.first + j) * kKeys + 16u * (lane & 7u);
+                if (lane >= 16 || key >= w.len) return 0.0f;
+                const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
                 if (page < 0 || (uint32_t)page >= p.pages) return lane < 8 ? -1.0f : 0.0f;
-                const uint64_t unit = (uint64_t)page * p.kv_heads + kv_head;
+                const uint64_t unit = (uint64_t)page * p.kv_heads + w.kv_head;
                 return lane < 8 ? p.k_scales[unit] : p.v_scales[unit] * (128.0f / v_top);
             };
             float scale_next = 0.0f, scale_now = 0.0f;
             if constexpr (kS8) scale_next = scale_of(0);
-            float m = -INFINITY, l = 0.0f;
+            float m = kLowest, l = 0.0f;
             // f16: P is kept times 2^7, which leaves f16 down to 2^-31 of the row's largest
             constexpr float kShift = kBF16 || kS8 ? 0.0f : 7.0f;
-            bool ok = true;
-            for (uint32_t j = 0; j < blocks; ++j) {
-                if (!warp_wait(&s_full[t], j & 1u)) {
+            for (uint32_t j = 0; j < w.blocks; ++j, ++done) {
+                if (!warp_wait(&s_full[t], done)) {
                     ok = false;
                     break;
                 }
@@ -259,18 +383,31 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(tS + 32u * i, sr[i]);
                 tmem_ld_wait();
+                if constexpr (!L::kAlias) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&s_free[t]);
+                }
                 float s[128];
 #pragma unroll
                 for (int i = 0; i < 128; ++i) s[i] = __uint_as_float(sr[i >> 5][i & 31]);
-                const uint32_t key0 = (first + j) * kKeys;
+                const uint32_t key0 = (w.first + j) * kKeys;
                 if constexpr (kS8) {
                     scale_now = scale_next;
-                    if (j + 1 < blocks) scale_next = scale_of(j + 1);
+                    if (j + 1 < w.blocks) scale_next = scale_of(j + 1);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float f = __shfl_sync(0xffffffffu, scale_now, i) * c;
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) s[16 * i + e] = f >= 0.0f ? s[16 * i + e] * f : -INFINITY;
+                        for (int e = 0; e < 16; e += 2) f2_mul(s[16 * i + e], s[16 * i + e + 1], s[16 * i + e], s[16 * i + e + 1], f, f);
+                    }
+                    if (__any_sync(0xffffffffu, scale_now < 0.0f)) {  // keys of no page of the cache
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (__shfl_sync(0xffffffffu, scale_now, i) < 0.0f) {
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) s[16 * i + e] = -INFINITY;
+                            }
                     }
                 }
                 if (key0 + kKeys > low) {
@@ -281,18 +418,26 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
                 float a[43];
 #pragma unroll
                 for (int i = 0; i < 42; ++i) a[i] = fmax3(s[3 * i], s[3 * i + 1], s[3 * i + 2]);
-                a[42] = fmaxf(s[126], s[127]);
+                a[42] = fmax3(s[126], s[127], s[127]);
 #pragma unroll
                 for (int i = 0; i < 14; ++i) a[i] = fmax3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) a[i] = fmax3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
                 float top = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[12], a[13]), a[42]);
                 if constexpr (!kS8) top = top == -INFINITY ? top : top * c;
+                if constexpr (!L::kAlias) {
+                    // P's columns, and O: the product of the block before is done
+                    if (j > 0 && !warp_wait(&pv_done[t], done - 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                }
                 const bool raise = top > m + kRaise;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float up = fmaxf(m, top);
-                    const float down = up == -INFINITY ? 1.0f : ex2_approx(m - up);
-                    if (j > 0) {  // O holds the blocks before: P V was issued before S
+                    const float down = ex2_approx(m - up);
+                    if (j > 0) {  // with P in S's columns, P V was issued before this S
 #pragma unroll 1
                         for (uint32_t k = 0; k < D / 8; ++k) {
                             uint32_t o[8];
@@ -307,11 +452,11 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
                     l *= down;
                     m = up;
                 }
-                const float off = kShift - (m == -INFINITY ? 0.0f : m);
+                const float off = kShift - m;
                 float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    uint32_t w[32];
+                    uint32_t x2[32];
                     float sv[4] = {1.0f, 1.0f, 1.0f, 1.0f};
                     if constexpr (kS8) {
 #pragma unroll
@@ -320,231 +465,423 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         float x = s[64 * h + 2 * i], y = s[64 * h + 2 * i + 1];
-                        if constexpr (kS8) {
-                            x = ex2_approx(x + off), y = ex2_approx(y + off);
-                            ls[(2 * i) & 3] += x, ls[(2 * i + 1) & 3] += y;
-                            const float f = sv[i / 8];
-                            w[i] = pack2<false>(x * f, y * f);
-                        } else {
-                            f2_fma(x, y, x, y, c, c, off, off);
-                            x = ex2_approx(x), y = ex2_approx(y);
-                            f2_add(ls[(2 * i) & 3], ls[(2 * i + 1) & 3], ls[(2 * i) & 3], ls[(2 * i + 1) & 3], x, y);
-                            w[i] = pack2<kBF16>(x, y);
-                        }
+                        if constexpr (kS8) f2_add(x, y, x, y, off, off);
+                        else f2_fma(x, y, x, y, c, c, off, off);
+                        if (i % 8 < kEmulated) exp2_pair(x, y);
+                        else x = ex2_approx(x), y = ex2_approx(y);
+                        f2_add(ls[(2 * i) & 3], ls[(2 * i + 1) & 3], ls[(2 * i) & 3], ls[(2 * i + 1) & 3], x, y);
+                        if constexpr (kS8) f2_mul(x, y, x, y, sv[i / 8], sv[i / 8]);
+                        x2[i] = pack2<kBF16>(x, y);
                     }
-                    tmem_st_32x32b_x32(tS + 32u * h, w);
+                    tmem_st_32x32b_x32(tP + 32u * h, x2);
                 }
                 l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+                if (top != top) l = top;  // a score is NaN: emulated exponentials would lose it
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            if (p.splits > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            if (ok) ok = warp_wait(o_full, 0);
+            if (!ok || !warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
-            if (ok) {
-                const float unit = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
-                const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
-                const float f = p.splits == 1 ? (l > 0.0f ? unit / l : 0.0f) : unit * back;
-                const uint64_t slot = live && p.splits > 1 ? part_at(p, where, kv_head, row, blockIdx.z) : 0;
-                const uint64_t at = live ? row_at(p, where, kv_head, row, p.out_batch, p.out_stride) : 0;
-                if (live && p.splits > 1) p.part_ml[slot] = make_float2(m, l * back);
+            if (m == kLowest) l = 0.0f;  // a row that sees nothing: its P is 0 or, emulated, 2^-126
+            const float unit_v = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
+            const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
+            const float f = l != 0.0f ? (p.splits == 1 ? unit_v / l : unit_v * back) : 0.0f;
+            const uint64_t slot = live && p.splits > 1 ? part_at(p, w.where, w.kv_head, row, w.split) : 0;
+            const uint64_t at = live ? row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride) : 0;
+            if (live && p.splits > 1) p.part_ml[slot] = make_float2(m, l * back);
 #pragma unroll 1
-                for (uint32_t k = 0; k < D / 32; ++k) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(tO + 32u * k, o);
-                    tmem_ld_wait();
-                    if (!live) continue;
+            for (uint32_t k = 0; k < D / 32; ++k) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(tO + 32u * k, o);
+                tmem_ld_wait();
+                if (!live) continue;
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        if (32 * k + i >= p.head_dim) continue;
-                        float x[8];
+                for (int i = 0; i < 32; i += 8) {
+                    if (32 * k + i >= p.head_dim) continue;
+                    float x[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = l > 0.0f ? __uint_as_float(o[i + e]) * f : 0.0f;
-                        if (p.splits > 1) {
-                            float4* to = reinterpret_cast<float4*>(p.part_o + slot * p.head_dim + 32 * k + i);
-                            to[0] = make_float4(x[0], x[1], x[2], x[3]);
-                            to[1] = make_float4(x[4], x[5], x[6], x[7]);
-                        } else if (p.out_kind == 0) {
-                            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + 32 * k + i);
-                            to[0] = make_float4(x[0], x[1], x[2], x[3]);
-                            to[1] = make_float4(x[4], x[5], x[6], x[7]);
-                        } else {
-                            uint32_t w[4];
+                    for (int e = 0; e < 8; ++e) x[e] = l != 0.0f ? __uint_as_float(o[i + e]) * f : 0.0f;
+                    if (p.splits > 1 || p.out_kind == 0) {
+                        float* to = p.splits > 1 ? p.part_o + slot * p.head_dim : static_cast<float*>(p.out) + at;
+                        float4* to4 = reinterpret_cast<float4*>(to + 32 * k + i);
+                        to4[0] = make_float4(x[0], x[1], x[2], x[3]);
+                        to4[1] = make_float4(x[4], x[5], x[6], x[7]);
+                    } else {
+                        uint32_t y[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                w[e] = p.out_kind == 1 ? pack2<true>(x[2 * e], x[2 * e + 1])
-                                                       : pack2<false>(x[2 * e], x[2 * e + 1]);
-                            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + 32 * k + i) =
-                                make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            y[e] = p.out_kind == 1 ? pack2<true>(x[2 * e], x[2 * e + 1])
+                                                   : pack2<false>(x[2 * e], x[2 * e + 1]);
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + 32 * k + i) =
+                            make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
-        } else if (t < tiles && live) {
-            // no key in reach
-            if (p.splits > 1) {
-                p.part_ml[part_at(p, where, kv_head, row, blockIdx.z)] = make_float2(-INFINITY, 0.0f);
-            } else {
-                const uint64_t at = row_at(p, where, kv_head, row, p.out_batch, p.out_stride);
-                const float zero[2] = {0.0f, 0.0f};
-                for (uint32_t i = 0; i < p.head_dim; i += 2) store_out(p, at + i, zero, 2);
-            }
+            tc_fence_before();  // O is read: the next unit's first product, after its P, may overwrite it
         }
-    } else if (warp == 8) {
-        // ----------------------------------------------------------- products
+    } else if (warp < kSoftmaxWarps + kIssuers<D, kS8>) {
+        // ------------------------------------------- products, and the next unit
+        // One thread issues, with everything but the waits unrolled: between its products the
+        // tensor cores may wait, as their queue holds a few (rolled up, 5 to 15% slower).
         constexpr uint32_t ab = kBF16 ? 1u : 0u;
-        constexpr uint32_t idesc_s = make_idesc(1u, ab, 128u, 128u);
+        const uint32_t idesc_s = make_idesc(1u, ab, 128u, 128u) | (p.scale_log2 < 0.0f ? 1u << 13 : 0u);  // or -Q
         constexpr uint32_t idesc_o = make_idesc(1u, ab, 128u, D) | (1u << 16);  // V is MN-major
+        constexpr uint32_t kStageDesc = L::kOperand >> 4;
+        const uint32_t kv_base = smem_addr(sKV) >> 4, q_all = (smem_addr(sQ) >> 4) | kDescK;
+        const uint32_t role = warp - kSoftmaxWarps;
+        uint32_t units = 0, stage = 0, phase = 0;  // stage and phase of the unit's next tile in the ring
+        uint32_t done0 = 0, done1 = 0;             // blocks of each tile before this unit
+        uint32_t turns = 0;                        // blocks of units with two tiles
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.err));
+            return mbar_wait(bar, parity & 1u, abort_flag, p.err);
         };
-        auto issue_s = [&](uint32_t t, uint32_t stage) {
-            const uint32_t q = smem_addr(sQ + t * L::kOperand), k = smem_addr(sKV + stage * L::kOperand);
+        auto next_stage = [&](uint32_t by) {
+            stage += by;
+            if (stage >= kStages) stage -= kStages, phase ^= 1u;
+        };
+        auto issue_s = [&](uint32_t t, uint32_t q, uint32_t st) {
+            q += t * kStageDesc;
+            const uint32_t k = kv_base + st * kStageDesc + kDescK, d = tmem + 128u * t;
+            umma_ss<false>(d, q, k, idesc_s);
 #pragma unroll
-            for (uint32_t kk = 0; kk < D / 16; ++kk) {
-                const uint32_t at = (kk / 4) * kAtom + 32u * (kk % 4);
-                umma<false>(tmem + 128u * t, smem_desc_sw128(q + at), smem_desc_sw128(k + at), idesc_s, kk ? 1u : 0u);
+            for (uint32_t kk = 1; kk < D / 16; ++kk) {
+                const uint32_t off = ((kk / 4) * kAtom + 32u * (kk % 4)) >> 4;
+                umma_ss<true>(d, q + off, k + off, idesc_s);
             }
             umma_commit(&s_full[t]);
         };
-        // K_j is tile 2j, V_j tile 2j + 1 of the ring
-        bool ok = true;
-        if (blocks) {
-            for (uint32_t t = 0; t < tiles && ok; ++t) ok = wait(&q_full[t], 0);
-            ok = ok && wait(&full[0], 0);
-            if (ok) {
-                tc_fence_after();
-                if (lane == 0) {
-                    for (uint32_t t = 0; t < tiles; ++t) issue_s(t, 0);
-                    umma_commit(&empty[0]);
-                    mma_issued = true;
-                }
-                __syncwarp();
+        auto issue_o = [&](uint32_t t, uint32_t st, uint32_t steps, uint32_t later) {
+            const uint32_t o = tmem + L::kO + t * D, pt = tmem + L::kP + t * L::kPStride;
+            const uint32_t v = kv_base + st * kStageDesc + kDescV;
+            if (steps == 8) {
+                umma_ts(o, pt, v, idesc_o, later);
+#pragma unroll
+                for (uint32_t kk = 1; kk < 8; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, 1u);
+            } else {
+                for (uint32_t kk = 0; kk < steps; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, later | kk);
             }
-        }
-        for (uint32_t j = 0; ok && j < blocks; ++j) {
-            const uint32_t nv = 2 * j + 1, nk = 2 * j + 2;
-            const uint32_t sv = nv % kStages, sk = nk % kStages;
-            const bool more = j + 1 < blocks;
-            const uint32_t valid = min(kKeys, len - (first + j) * kKeys);
-            const uint32_t steps = (valid + 15u) / 16u;
-            for (uint32_t t = 0; t < tiles && ok; ++t) {
-                if (t == 0) {
-                    ok = wait(&full[sv], (nv / kStages) & 1u);
-                    if (ok && !kS8 && (valid & 15u)) {
-                        // rows of V behind the last key, up to the product's end
-                        uint8_t* v = sKV + sv * L::kOperand;
-                        for (uint32_t i = lane; i < (16u - (valid & 15u)) * (D / 8); i += 32) {
-                            const uint32_t row = valid + i / (D / 8);
-                            *reinterpret_cast<uint4*>(v + chunk_at(row, i % (D / 8))) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_async_smem();
-                        __syncwarp();
-                    }
+        };
+        // rows of V behind the last key, up to the product's end
+        auto clear_tail = [&](uint32_t st, uint32_t valid) {
+            uint8_t* v = sKV + st * L::kOperand;
+#pragma unroll 1
+            for (uint32_t i = 0; i < (16u - (valid & 15u)) * (D / 8); ++i)
+                *reinterpret_cast<uint4*>(v + chunk_at(valid + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
+            fence_async_smem();
+        };
+        uint32_t u = blockIdx.x;
+        for (uint32_t iter = 0;; ++iter) {
+            if (iter && !next_unit(iter - 1, u)) break;
+            // ask for the next unit once every warp has read the response before the last
+            const uint32_t slot = iter & 1u;
+            if (role == 0 && !warp_wait(&unit_empty[slot], ((iter >> 1) & 1u) ^ 1u)) break;
+            if (role == 0 && lane == 0) {
+                fence_async_smem();
+                mbar_arrive_expect_tx(&unit_full[slot], 16);
+                request_unit(&response[slot], &unit_full[slot]);
+            }
+            __syncwarp();
+            const Unit w = unit_at(p, n, u);
+            if (!w.blocks) continue;
+            const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
+            const uint32_t tiles = w.tiles, blocks = w.blocks;
+            const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
+            bool ok = true;
+            if (lane == 0) {
+                mma_issued = true;
+                const uint32_t t0 = kIssuers<D, kS8> == 2 ? role : 0;
+                const uint32_t t1 = kIssuers<D, kS8> == 2 ? min(t0 + 1, tiles) : tiles;
+                const bool take_turns = kTurns<D> && kIssuers<D, kS8> == 2 && tiles == 2;
+                ok = wait(&q_full[qb], units / kQBufs) && wait(&full[stage], phase);
+#pragma unroll 1
+                for (uint32_t t = t0; t < t1 && ok; ++t) {
+                    const uint32_t before = t ? done1 : done0;
+                    if (!L::kAlias && before) ok = wait(&s_free[t], before - 1);
+                    tc_fence_after();
+                    if (ok) issue_s(t, q, stage);
                 }
-                ok = ok && wait(&p_full[t], j & 1u);
-                if (ok && more && t == 0) ok = wait(&full[sk], (nk / kStages) & 1u);
-                if (!ok) break;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t v = smem_addr(sKV + sv * L::kOperand);
-                    for (uint32_t kk = 0; kk < steps; ++kk)
-                        umma_ts(tmem + L::kO + t * D, tmem + 128u * t + 8u * kk, desc_v(v + kk * 2048u), idesc_o,
-                                (j | kk) ? 1u : 0u);
-                    if (t + 1 == tiles) umma_commit(&empty[sv]);
+                if (t0 < t1) {
+                    umma_commit(&empty[stage]);
+                    if (blocks == 1) umma_commit(&q_empty[qb]);
+                } else if (ok) {  // no rows of this tile: its stages are released as they are filled
+                    mbar_arrive(&empty[stage]);
+                    mbar_arrive(&q_empty[qb]);
+                }
+                next_stage(1);
+#pragma unroll 1
+                for (uint32_t j = 0; ok && j < blocks; ++j) {
+                    const bool more = j + 1 < blocks;
+                    const uint32_t sv = stage;
+                    ok = wait(&full[sv], phase);
+                    next_stage(1);
+                    const uint32_t sk = stage;
                     if (more) {
-                        issue_s(t, sk);
-                        if (t + 1 == tiles) umma_commit(&empty[sk]);
-                    } else if (t + 1 == tiles) {
-                        umma_commit(o_full);
+                        ok = ok && wait(&full[sk], phase);
+                        next_stage(1);
+                    }
+                    if (t0 >= t1) {
+                        if (!ok) break;
+                        mbar_arrive(&empty[sv]);
+                        if (more) mbar_arrive(&empty[sk]);
+                        continue;
+                    }
+                    const uint32_t valid = more ? kKeys : last_keys;
+                    if (ok && !kS8 && (valid & 15u)) clear_tail(sv, valid);
+                    // S of the next block: beside this block's softmax where P has its own columns
+                    if (!L::kAlias && more) {
+#pragma unroll 1
+                        for (uint32_t t = t0; t < t1 && ok; ++t) {
+                            ok = wait(&s_free[t], (t ? done1 : done0) + j);
+                            tc_fence_after();
+                            if (ok) issue_s(t, q, sk);
+                        }
+                        umma_commit(&empty[sk]);
+                        if (j + 2 == blocks) umma_commit(&q_empty[qb]);
+                    }
+#pragma unroll 1
+                    for (uint32_t t = t0; t < t1 && ok; ++t) {
+                        ok = wait(&p_full[t], (t ? done1 : done0) + j);
+                        // the tiles' products one after the other, not interleaved: tile 0 of
+                        // block j, tile 1 of block j, tile 0 of block j + 1
+                        if (take_turns && ok && (t || turns + j)) ok = wait(&turn[t], t ? turns + j : turns + j - 1);
+                        tc_fence_after();
+                        if (!ok) break;
+                        issue_o(t, sv, (valid + 15u) / 16u, j);
+                        if (L::kAlias && more) issue_s(t, q, sk);
+                        if (take_turns) mbar_arrive(&turn[t ^ 1u]);
+                        if (!L::kAlias) umma_commit(&pv_done[t]);
+                        if (!more) umma_commit(&o_full[t]);
+                    }
+                    umma_commit(&empty[sv]);
+                    if (L::kAlias && more) {
+                        umma_commit(&empty[sk]);
+                        if (j + 2 == blocks) umma_commit(&q_empty[qb]);
                     }
                 }
-                __syncwarp();
             }
+            done0 += blocks;
+            if (tiles == 2) done1 += blocks, turns += blocks;
+            ++units;
+            __syncwarp();
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
         }
     } else if constexpr (!kS8) {
-        // ---------------------------------------------------------------- TMA
-        if (lane == 0) {
-            const int batch = p.k_batch ? (int)where.seq : 0, v_batch = p.v_batch ? (int)where.seq : 0;
-            for (uint32_t n = 0; n < 2 * blocks; ++n) {
-                const uint32_t st = n % kStages;
-                if (*abort_flag || !mbar_wait(&empty[st], ((n / kStages) & 1u) ^ 1u, abort_flag, p.err)) break;
-                mbar_arrive_expect_tx(&full[st], L::kOperand);
-                const int key0 = (int)((first + n / 2) * kKeys);
+        uint32_t ring = 0, units = 0;
+        if (warp == 10) {
+            // ------------------------------------------------------------ TMA
+            uint32_t u = blockIdx.x;
+            for (uint32_t iter = 0;; ++iter) {
+                if (iter && !next_unit(iter - 1, u)) break;
+                const Unit w = unit_at(p, n, u);
+                bool ok = true;
+                if (lane == 0) {
+                    const int k_batch = p.k_batch ? (int)w.where.seq : 0, v_batch = p.v_batch ? (int)w.where.seq : 0;
+                    for (uint32_t i = 0; i < 2 * w.blocks; ++i) {
+                        const uint32_t at = ring + i, st = at % kStages;
+                        if (*abort_flag || !mbar_wait(&empty[st], ((at / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+                            ok = false;
+                            break;
+                        }
+                        mbar_arrive_expect_tx(&full[st], L::kOperand);
+                        const int key0 = (int)((w.first + i / 2) * kKeys);
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h)
-                    tma_load_4d(sKV + st * L::kOperand + h * kAtom, n & 1 ? &tm_v : &tm_k, &full[st], 64 * h,
-                                (int)kv_head, key0, n & 1 ? v_batch : batch);
+                        for (int h = 0; h < D / 64; ++h)
+                            tma_load_4d(sKV + st * L::kOperand + h * kAtom, i & 1 ? &tm_v : &tm_k, &full[st], 64 * h,
+                                        (int)w.kv_head, key0, i & 1 ? v_batch : k_batch);
+                    }
+                }
+                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+                ring += 2 * w.blocks;
+            }
+        } else if (warp == 11) {
+            // -------------------------------------------------------------- Q
+            uint32_t u = blockIdx.x;
+            for (uint32_t iter = 0;; ++iter) {
+                if (iter && !next_unit(iter - 1, u)) break;
+                const Unit w = unit_at(p, n, u);
+                if (!w.blocks) continue;
+                const uint32_t qb = units % kQBufs;
+                if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
+                ++units;
+                uint8_t* to = sQ + qb * 2 * L::kOperand;
+                if (n.q_box) {
+                    // 128 rows are q_box tokens of the group's heads
+                    if (lane == 0) {
+                        mbar_arrive_expect_tx(&q_full[qb], w.tiles * L::kOperand);
+                        const int batch = p.q_batch ? (int)w.where.seq : 0;
+                        for (uint32_t t = 0; t < w.tiles; ++t)
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h)
+                                tma_load_4d(to + t * L::kOperand + h * kAtom, &tm_q, &q_full[qb], 64 * h,
+                                            (int)(w.kv_head * p.group), (int)((w.where.tile * 2 + t) * n.q_box), batch);
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                const uint32_t rows = w.tiles * kTileRows;
+#pragma unroll 1
+                for (uint32_t i = lane; i < rows * (D / 8); i += 32) {
+                    const uint32_t r = i / (D / 8), chunk = i % (D / 8), row = w.row0 + r;
+                    const bool read = row < w.where.rows && 8 * chunk < p.head_dim;
+                    const uint16_t* from = static_cast<const uint16_t*>(p.q) +
+                                           (read ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) + 8 * chunk : 0);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                     smem_addr(to + (r / kTileRows) * L::kOperand + chunk_at(r % kTileRows, chunk))),
+                                 "l"(from), "r"(read ? 16u : 0u)
+                                 : "memory");
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[qb]);
             }
         }
     } else {
         // -------------------------------------------------------------- codes
         // a thread converts 16 dims of a key at a time
         constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
-        constexpr uint32_t kLoads = (kKeys * kParts + kStep - 1) / kStep;
-        const uint32_t i0 = threadIdx.x - (kSoftmaxThreads + 32);
+        constexpr uint32_t kHalf = kKeys / 2, kLoads = (kHalf * kParts + kStep - 1) / kStep;
+        const uint32_t i0 = threadIdx.x - 9 * 32;
         const uint32_t in_page = (1u << p.page_shift) - 1;
-        // lane i < 8 has the page of keys 16i .. 16i + 15 of a block, fetched a block ahead
-        auto page_of = [&](uint32_t j) -> int32_t {
-            const uint32_t key = (first + j) * kKeys + 16u * (lane & 7u);
-            if (key >= len) return -1;
-            const int32_t page = p.page_table[(uint64_t)where.seq * p.table_stride + (key >> p.page_shift)];
-            if (page < 0 || (uint32_t)page >= p.pages) {
-                atomicExch(p.err, 3);
-                return -1;
-            }
-            return page;
-        };
-        int32_t page_now = -1, page_next = blocks ? page_of(0) : -1;
-        uint4 x[kLoads];
-        auto load = [&](uint32_t n) {
-            const int8_t* codes = static_cast<const int8_t*>(n & 1 ? p.v : p.k);
-            if (!(n & 1)) {
-                page_now = page_next;
-                if (n / 2 + 1 < blocks) page_next = page_of(n / 2 + 1);
-            }
+        uint32_t ring = 0, units = 0;
+        bool ok = true;
+        uint32_t u = blockIdx.x;
+        for (uint32_t iter = 0; ok; ++iter) {
+            if (iter && !next_unit(iter - 1, u)) break;
+            const Unit w = unit_at(p, n, u);
+            if (!w.blocks) continue;
+            // lane i < 8 has the page of keys 16i .. 16i + 15 of a block, fetched a block ahead
+            auto page_of = [&](uint32_t j) -> int32_t {
+                const uint32_t key = (w.first + j) * kKeys + 16u * (lane & 7u);
+                if (key >= w.len) return -1;
+                const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
+                if (page < 0 || (uint32_t)page >= p.pages) {
+                    atomicExch(p.err, 3);
+                    return -1;
+                }
+                return page;
+            };
+            int32_t page_now = -1, page_next = page_of(0);
+            // half an operand (64 keys) in each buffer, loaded while the other is converted;
+            // halves 4j, 4j + 1 are K_j, 4j + 2 and 4j + 3 V_j
+            uint4 x[2][kLoads];
+            auto load = [&](uint32_t h, uint4 (&x)[kLoads]) {
+                const int8_t* codes = static_cast<const int8_t*>(h & 2 ? p.v : p.k);
+                if (!(h & 3)) {
+                    page_now = page_next;
+                    if (h / 4 + 1 < w.blocks) page_next = page_of(h / 4 + 1);
+                }
 #pragma unroll
-            for (uint32_t k = 0; k < kLoads; ++k) {
-                const uint32_t i = i0 + kStep * k, key = i / kParts, part = i % kParts;
-                const int32_t page = __shfl_sync(0xffffffffu, page_now, (key >> 4) & 7);
-                x[k] = make_uint4(0, 0, 0, 0);
-                if (page >= 0 && key < kKeys && 16 * part < p.head_dim)
-                    x[k] = *reinterpret_cast<const uint4*>(
-                        codes + ((((uint64_t)page * p.kv_heads + kv_head) << p.page_shift) +
-                                 (((first + n / 2) * kKeys + key) & in_page)) * p.head_dim + 16 * part);
+                for (uint32_t k = 0; k < kLoads; ++k) {
+                    const uint32_t at = i0 + kStep * k, in_half = at / kParts, part = at % kParts;
+                    const uint32_t key = in_half + (h & 1) * kHalf;
+                    const int32_t page = __shfl_sync(0xffffffffu, page_now, (key >> 4) & 7);
+                    x[k] = make_uint4(0, 0, 0, 0);
+                    if (page >= 0 && in_half < kHalf && 16 * part < p.head_dim)
+                        x[k] = *reinterpret_cast<const uint4*>(
+                            codes + ((((uint64_t)page * p.kv_heads + w.kv_head) << p.page_shift) +
+                                     (((w.first + h / 4) * kKeys + key) & in_page)) * p.head_dim + 16 * part);
+                }
+            };
+            load(0, x[0]);
+            load(1, x[1]);
+            // the largest V scale of the keys in reach
+            float v_top = 1e-30f;
+            const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
+            for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
+                const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
+                if (page >= 0 && (uint32_t)page < p.pages)
+                    v_top = fmaxf(v_top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
             }
-        };
-        if (blocks) load(0);
-        for (uint32_t n = 0; n < 2 * blocks; ++n) {
-            const uint32_t st = n % kStages;
-            if (!__all_sync(0xffffffffu, mbar_wait(&empty[st], ((n / kStages) & 1u) ^ 1u, abort_flag, p.err))) break;
-            uint8_t* to = sKV + st * L::kOperand;
+            v_top = warp_max(v_top);
+            // rows of Q, brought into f16's range by a power of two each: a warp to a row
+            const uint32_t qb = units % kQBufs;
+            if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
+            int8_t* back = s_back + units % L::kBackSlots * 2 * kTileRows;
+            if (i0 == 0) s_top[units % L::kBackSlots] = v_top;
+            uint8_t* to_q = sQ + qb * 2 * L::kOperand;
+            ++units;
+            for (uint32_t r0 = i0 / 32; r0 < w.tiles * kTileRows; r0 += 4 * kConverters) {
+                // a lane has D / 32 values of each of four rows
+                uint32_t q2[4][D / 64];
 #pragma unroll
-            for (uint32_t k = 0; k < kLoads; ++k) {
-                const uint32_t i = i0 + kStep * k, key = i / kParts, part = i % kParts;
-                if (key >= kKeys) continue;
-                const uint32_t w4[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u,
-                                        x[k].w ^ 0x80808080u};
-                *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part)) =
-                    make_uint4(codes_lo(w4[0]), codes_hi(w4[0]), codes_lo(w4[1]), codes_hi(w4[1]));
-                *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part + 1)) =
-                    make_uint4(codes_lo(w4[2]), codes_hi(w4[2]), codes_lo(w4[3]), codes_hi(w4[3]));
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t row = w.row0 + r0 + kConverters * e;
+                    const bool live = r0 + kConverters * e < w.tiles * kTileRows && row < w.where.rows;
+                    const uint16_t* q = static_cast<const uint16_t*>(p.q) +
+                                        (live ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) : 0);
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k)
+                        q2[e][k] = live && D / 32 * lane + 2 * k < p.head_dim
+                                       ? *reinterpret_cast<const uint32_t*>(q + D / 32 * lane + 2 * k)
+                                       : 0u;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t r = r0 + kConverters * e;
+                    if (r >= w.tiles * kTileRows) break;
+                    float most = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k) {
+                        const float2 y = unpack2(q2[e][k], p.q_bf16);
+                        most = fmax3(most, fabsf(y.x), fabsf(y.y));
+                    }
+                    most = warp_max(most);
+                    int ex = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
+                    ex = max(-120, min(120, ex));
+                    const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
+                    if (lane == 0) back[r] = (int8_t)ex;
+#pragma unroll
+                    for (int k = 0; k < D / 64; ++k) {
+                        const float2 y = unpack2(q2[e][k], p.q_bf16);
+                        const uint32_t dim = D / 32 * lane + 2 * k;
+                        *reinterpret_cast<uint32_t*>(to_q + (r / kTileRows) * L::kOperand +
+                                                     chunk_at(r % kTileRows, dim / 8) + 2 * (dim % 8)) =
+                            pack2<false>(y.x * up, y.y * up);
+                    }
+                }
             }
             fence_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[st]);
-            if (n + 1 < 2 * blocks) load(n + 1);
+            if (lane == 0) mbar_arrive(&q_full[qb]);
+            auto convert = [&](uint32_t h, uint4 (&x)[kLoads]) -> bool {
+                const uint32_t at = ring + h / 2, st = at % kStages;
+                if (!(h & 1) && !warp_wait(&empty[st], (at / kStages) ^ 1u)) return false;
+                uint8_t* to = sKV + st * L::kOperand;
+#pragma unroll
+                for (uint32_t k = 0; k < kLoads; ++k) {
+                    const uint32_t at16 = i0 + kStep * k, in_half = at16 / kParts, part = at16 % kParts;
+                    const uint32_t key = in_half + (h & 1) * kHalf;
+                    if (in_half >= kHalf) continue;
+                    const uint32_t w4[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u,
+                                            x[k].w ^ 0x80808080u};
+                    *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part)) =
+                        make_uint4(codes_lo(w4[0]), codes_hi(w4[0]), codes_lo(w4[1]), codes_hi(w4[1]));
+                    *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part + 1)) =
+                        make_uint4(codes_lo(w4[2]), codes_hi(w4[2]), codes_lo(w4[3]), codes_hi(w4[3]));
+                }
+                if (h & 1) {
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[st]);
+                }
+                if (h + 2 < 4 * w.blocks) load(h + 2, x);
+                return true;
+            };
+            for (uint32_t h = 0; ok && h < 4 * w.blocks; h += 2) ok = convert(h, x[0]) && convert(h + 1, x[1]);
+            ring += 2 * w.blocks;
         }
     }
 
     __syncthreads();
     if (*abort_flag) {
-        if (warp == 8 && lane == 0 && mma_issued) {
-            umma_commit(drain);
+        if (warp >= kSoftmaxWarps && warp < kSoftmaxWarps + kIssuers<D, kS8> && lane == 0 && mma_issued) {
+            uint64_t* d = &drain[warp - kSoftmaxWarps];
+            umma_commit(d);
             const unsigned long long t0 = globaltimer();
-            while (!mbar_try_wait(smem_addr(drain), 0) && globaltimer() - t0 < 100000000ull) {
+            while (!mbar_try_wait(smem_addr(d), 0) && globaltimer() - t0 < 100000000ull) {
             }
         }
         if (threadIdx.x == 0) {  // copies in flight land before the block's memory is given back
@@ -554,11 +891,12 @@ __global__ void __launch_bounds__((Layout<D, kS8>::kThreads), 1)
         }
         __syncthreads();
     }
-    if (warp == 8) {
+    if (warp == kSoftmaxWarps) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
 }
+
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
@@ -578,9 +916,25 @@ bool encode_keys(CUtensorMap& tm, const RowsParams& p, const void* rows, uint64_
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// q [batch][queries][q_heads][head_dim] as boxes of 64 dims x the heads of a group x
+// as many tokens as make 128 rows.
+bool encode_queries(CUtensorMap& tm, const RowsParams& p, uint32_t tokens, bool bf16) {
+    const uint64_t row = (uint64_t)p.kv_heads * p.group * p.head_dim;
+    const bool batches = p.q_batch && p.sequences > 1;
+    const cuuint64_t dims[4] = {p.head_dim, (cuuint64_t)p.kv_heads * p.group, p.queries, batches ? p.sequences : 1u};
+    const cuuint64_t strides[3] = {p.head_dim * 2ull, (p.queries > 1 ? p.q_stride : row) * 2,
+                                   (batches ? p.q_batch : row) * 2};
+    const cuuint32_t box[4] = {64, p.group, tokens, 1}, each[4] = {1, 1, 1, 1};
+    return g_encode(&tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                    const_cast<void*>(p.q), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool kS8, bool kBF16>
-int start(const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, uint32_t slots, cudaStream_t st) {
-    using L = Layout<D, kS8>;
+int start(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, const TilesParams& n, uint32_t units,
+          cudaStream_t st) {
+    using L = Layout<D>;
     auto kernel = attention_tiles_kernel<D, kS8, kBF16>;
     static std::atomic<uint64_t> configured;  // one bit per device ordinal
     int dev = 0;
@@ -592,14 +946,15 @@ int start(const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, uint3
             return set_error(DAV2CUDA_LAUNCH_FAILED, "attention: cannot set shared memory size");
         mark_configured(configured, dev);
     }
-    kernel<<<dim3(slots, p.kv_heads, p.splits), L::kThreads, L::kSmem, st>>>(k, v, p);
+    kernel<<<units, kThreads, L::kSmem, st>>>(q, k, v, p, n);
     return check_launch("attention_tiles");
 }
 
 }  // namespace
 
 int launch_attention_tiles(const RowsParams& p, uint32_t slots, bool s8, bool bf16, cudaStream_t st) {
-    CUtensorMap k{}, v{};
+    CUtensorMap q{}, k{}, v{};
+    TilesParams n{};
     if (!s8 && p.max_length) {
         std::call_once(g_encode_once, [] {
             void* fn = nullptr;
@@ -611,11 +966,21 @@ int launch_attention_tiles(const RowsParams& p, uint32_t slots, bool s8, bool bf
         if (!g_encode) return set_error(DAV2CUDA_INTERNAL_ERROR, "cuTensorMapEncodeTiled unavailable");
         if (!encode_keys(k, p, p.k, p.k_stride, p.k_batch, bf16) || !encode_keys(v, p, p.v, p.v_stride, p.v_batch, bf16))
             return set_error(DAV2CUDA_INVALID_ARGUMENT, "attention: tensor map encoding failed");
+        // any other group: rows that a warp copies
+        if (kTileRows % p.group == 0 && encode_queries(q, p, kTileRows / p.group, bf16)) n.q_box = kTileRows / p.group;
     }
+    const uint64_t heads = (uint64_t)p.kv_heads * p.splits, rows = (uint64_t)p.queries * p.group;
+    n.slots = slots;
+    n.full_tiles = (uint32_t)(rows / (2 * kTileRows));
+    const uint64_t full_units = p.query_begin ? 0 : heads * p.sequences * n.full_tiles;
+    const uint64_t units = p.query_begin ? heads * slots
+                                         : full_units + (rows % (2 * kTileRows) ? heads * p.sequences : 0);
+    if (units > 0x7FFFFFFFu) return set_error(DAV2CUDA_INVALID_ARGUMENT, "attention: too many row tiles");
+    n.full_units = (uint32_t)full_units;
     const bool small = p.head_dim <= 64;
-    if (s8) return small ? start<64, true, false>(k, v, p, slots, st) : start<128, true, false>(k, v, p, slots, st);
-    if (bf16) return small ? start<64, false, true>(k, v, p, slots, st) : start<128, false, true>(k, v, p, slots, st);
-    return small ? start<64, false, false>(k, v, p, slots, st) : start<128, false, false>(k, v, p, slots, st);
+    if (s8) return small ? start<64, true, false>(q, k, v, p, n, (uint32_t)units, st) : start<128, true, false>(q, k, v, p, n, (uint32_t)units, st);
+    if (bf16) return small ? start<64, false, true>(q, k, v, p, n, (uint32_t)units, st) : start<128, false, true>(q, k, v, p, n, (uint32_t)units, st);
+    return small ? start<64, false, false>(q, k, v, p, n, (uint32_t)units, st) : start<128, false, false>(q, k, v, p, n, (uint32_t)units, st);
 }
 
 }  // namespace dav2cuda

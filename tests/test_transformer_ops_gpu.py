@@ -370,6 +370,24 @@ def test_cross_attention_sharp_and_flat(cuda, dav2lib, queries, spread):
     check_cross(dav2lib, 2, queries, 900, 4, 2, 64, [900, 600], 1, 0, spread=spread)
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+@pytest.mark.parametrize("queries", [1, 300])
+def test_attention_scale_zero_and_negative(cuda, dav2lib, scale, queries):
+    g = gen(15)
+    q, k, v = (randn(g, 2, n, 4, 64, dtype=torch.float16) for n in (queries, 333, 333))
+    out, lengths = torch.empty(2, queries, 4, 64, device="cuda"), ints([333, 190])
+    cross(dav2lib, q, k, v, lengths, scale, out)
+    done(dav2lib)
+    want, bound = ref.cross_attention(q, k, v, [333, 190], scale, 2, 0)
+    assert ref.outside(out, want, bound) <= 1
+    c = Cache(g, [333, 500], 2, 64, 32)
+    q = q.flatten(0, 1)
+    out = torch.empty(2 * queries, 4, 64, device="cuda")
+    attend_cache(dav2lib, c, q, [333, 500], [0, queries, 2 * queries], True, out, scale)
+    want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, [333, 500], [0, queries, 2 * queries], scale, True, 0)
+    assert ref.outside(out, want, bound) <= 1
+
+
 def test_cross_attention_rows_in_any_order(cuda, dav2lib):
     """Batch and token strides of slices, q as a part of packed rows, k and v from different tensors."""
     g = gen(2)
