@@ -65,22 +65,26 @@ constexpr float kLowest = -3.402823466e38f;
 // 5477, 16 heads of 128, 233, 229, 237, 231, 268 us.
 constexpr int kEmulated = 2;
 
-template <int D>
+template <int D, bool kS8>
 struct Layout {
     static constexpr uint32_t kOperand = D / 64 * kAtom;   // bytes of 128 rows
     static constexpr uint32_t kQBufs = D == 64 ? 2 : 1;    // Q of this unit and the next
-    static constexpr uint32_t kStages = D == 64 ? 8 : 5;    // K or V tiles in flight
+    static constexpr uint32_t kStages = kS8 ? (D == 64 ? 5 : 3) : (D == 64 ? 8 : 5);  // K or V tiles of 16 bits
+    static constexpr uint32_t kRaw = kS8 ? 4 : 0;          // tiles of codes in flight
+    static constexpr uint32_t kRawBytes = D * kKeys;
     static constexpr uint32_t kBackSlots = 2 * kQBufs;     // codes: units whose row factors are kept
     static constexpr uint32_t kBars = 512;                  // bytes of barriers
     static constexpr uint32_t kSmem =
-        (2 * kQBufs + kStages) * kOperand + kBars + kBackSlots * 2 * kTileRows;
+        (2 * kQBufs + kStages) * kOperand + kRaw * kRawBytes + kBars + (kS8 ? kBackSlots * 2 * kTileRows : 0);
     // Tensor memory columns: S_0, S_1, O_0, O_1, and at D = 64 P_0, P_1; at D = 128,
     // where S and O fill it, P_t takes the first half of S_t.
     static constexpr bool kAlias = D == 128;
     static constexpr uint32_t kO = 256;
     static constexpr uint32_t kP = kAlias ? 0 : 384, kPStride = kAlias ? 128 : 64;
 };
-static_assert(Layout<128>::kSmem <= 232448 && Layout<64>::kSmem <= 232448, "shared memory above the per-block limit");
+static_assert(Layout<128, false>::kSmem <= 232448 && Layout<64, false>::kSmem <= 232448 &&
+                  Layout<128, true>::kSmem <= 232448 && Layout<64, true>::kSmem <= 232448,
+              "shared memory above the per-block limit");
 
 struct TilesParams {
     uint32_t q_box;  // Q by TMA: tokens of a 128-row box (0: by a warp)
@@ -238,13 +242,14 @@ template <int D, bool kS8, bool kBF16>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                            const __grid_constant__ CUtensorMap tm_v, const RowsParams p, const TilesParams n) {
-    using L = Layout<D>;
+    using L = Layout<D, kS8>;
     constexpr uint32_t kStages = L::kStages;
     constexpr uint32_t kQBufs = L::kQBufs;
     extern __shared__ uint8_t smem[];
     uint8_t* sQ = smem;                        // [tile]
     uint8_t* sKV = smem + 2 * kQBufs * L::kOperand;  // [stage]
-    uint8_t* control = sKV + kStages * L::kOperand;
+    uint8_t* sRaw = sKV + kStages * L::kOperand;     // [raw slot] codes, rows of head_dim bytes
+    uint8_t* control = sRaw + L::kRaw * L::kRawBytes;
     uint4* response = reinterpret_cast<uint4*>(control);  // [2]
     uint64_t* full = reinterpret_cast<uint64_t*>(response + 2);  // [stage]
     uint64_t* empty = full + kStages;    // [stage]
@@ -259,11 +264,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* unit_empty = unit_full + 2;  // [response]
     uint64_t* turn = unit_empty + 2;     // [tile]
     uint64_t* drain = turn + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
+    uint64_t* raw_full = drain + 2;      // [raw slot]
+    uint64_t* raw_empty = raw_full + 4;  // [raw slot]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     float* s_top = reinterpret_cast<float*>(tmem_slot + 4);        // codes: [slot] the largest V scale
     int8_t* s_back = reinterpret_cast<int8_t*>(control + L::kBars);  // codes: [slot][row] powers of two of Q
-    static_assert(32 + 8 * (2 * kStages + 22) + 32 <= L::kBars, "barriers overflow their part");
+    static_assert(32 + 8 * (2 * kStages + 30) + 32 <= L::kBars, "barriers overflow their part");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if ((smem_addr(smem) & 1023u) != 0) {  // the 128-byte swizzle needs 1 KB aligned tiles
@@ -286,6 +293,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&q_empty[t], kIssuers<D, kS8>);
             mbar_init(&unit_full[t], 1);
             mbar_init(&unit_empty[t], kSoftmaxWarps + kIssuers<D, kS8> + (kS8 ? kConverters : 2));  // warps at work
+        }
+        for (uint32_t i = 0; kS8 && i < 4; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_empty[i], kConverters);
         }
         mbar_init(&drain[0], 1);
         mbar_init(&drain[1], 1);
@@ -740,9 +751,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // -------------------------------------------------------------- codes
-        // a thread converts 16 dims of a key at a time
+        // Warp 9 keeps kRaw tiles of codes under way from the pages (a page's tokens of a head
+        // are one run of bytes, copied in one piece); the three warps turn each into a 16-bit
+        // tile, 16 dims of a key at a time.
         constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
-        constexpr uint32_t kHalf = kKeys / 2, kLoads = (kHalf * kParts + kStep - 1) / kStep;
         const uint32_t i0 = threadIdx.x - 9 * 32;
         const uint32_t in_page = (1u << p.page_shift) - 1;
         uint32_t ring = 0, units = 0;
@@ -752,10 +764,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (iter && !next_unit(iter - 1, u)) break;
             const Unit w = unit_at(p, n, u);
             if (!w.blocks) continue;
-            // lane i < 8 has the page of keys 16i .. 16i + 15 of a block, fetched a block ahead
+            // lanes 0 to 7 have the page of their piece of a block, fetched a block ahead
+            const uint32_t piece = min(1u << p.page_shift, kKeys);
             auto page_of = [&](uint32_t j) -> int32_t {
-                const uint32_t key = (w.first + j) * kKeys + 16u * (lane & 7u);
-                if (key >= w.len) return -1;
+                const uint32_t in_block = lane * piece, key = (w.first + j) * kKeys + in_block;
+                if (in_block >= kKeys || key >= w.len) return -1;
                 const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
                 if (page < 0 || (uint32_t)page >= p.pages) {
                     atomicExch(p.err, 3);
@@ -763,30 +776,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return page;
             };
-            int32_t page_now = -1, page_next = page_of(0);
-            // half an operand (64 keys) in each buffer, loaded while the other is converted;
-            // halves 4j, 4j + 1 are K_j, 4j + 2 and 4j + 3 V_j
-            uint4 x[2][kLoads];
-            auto load = [&](uint32_t h, uint4 (&x)[kLoads]) {
-                const int8_t* codes = static_cast<const int8_t*>(h & 2 ? p.v : p.k);
-                if (!(h & 3)) {
+            int32_t page_now = -1, page_next = i0 < 32 ? page_of(0) : -1;
+            // Starts the copies of tile i (K_j: 2j, V_j: 2j + 1). Keys of no page, and past the
+            // end, keep what the slot holds: any byte is a finite code, and they weigh nothing.
+            auto fetch = [&](uint32_t i) -> bool {
+                const uint32_t at = ring + i, slot = at % L::kRaw;
+                if (!warp_wait(&raw_empty[slot], (at / L::kRaw) ^ 1u)) return false;
+                if (!(i & 1)) {
                     page_now = page_next;
-                    if (h / 4 + 1 < w.blocks) page_next = page_of(h / 4 + 1);
+                    if (i / 2 + 1 < w.blocks) page_next = page_of(i / 2 + 1);
                 }
-#pragma unroll
-                for (uint32_t k = 0; k < kLoads; ++k) {
-                    const uint32_t at = i0 + kStep * k, in_half = at / kParts, part = at % kParts;
-                    const uint32_t key = in_half + (h & 1) * kHalf;
-                    const int32_t page = __shfl_sync(0xffffffffu, page_now, (key >> 4) & 7);
-                    x[k] = make_uint4(0, 0, 0, 0);
-                    if (page >= 0 && in_half < kHalf && 16 * part < p.head_dim)
-                        x[k] = *reinterpret_cast<const uint4*>(
-                            codes + ((((uint64_t)page * p.kv_heads + w.kv_head) << p.page_shift) +
-                                     (((w.first + h / 4) * kKeys + key) & in_page)) * p.head_dim + 16 * part);
+                const uint32_t bytes = piece * p.head_dim;
+                const uint32_t live = __popc(__ballot_sync(0xffffffffu, page_now >= 0));
+                if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], live * bytes);
+                __syncwarp();
+                if (page_now >= 0) {
+                    const uint32_t key = (w.first + i / 2) * kKeys + lane * piece;
+                    const int8_t* from =
+                        static_cast<const int8_t*>(i & 1 ? p.v : p.k) +
+                        ((((uint64_t)page_now * p.kv_heads + w.kv_head) << p.page_shift) + (key & in_page)) * p.head_dim;
+                    asm volatile(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                            smem_addr(sRaw + slot * L::kRawBytes + lane * bytes)),
+                        "l"(from), "r"(bytes), "r"(smem_addr(&raw_full[slot]))
+                        : "memory");
                 }
+                __syncwarp();
+                return true;
             };
-            load(0, x[0]);
-            load(1, x[1]);
+            const uint32_t count = 2 * w.blocks;
+            if (i0 < 32)
+                for (uint32_t i = 0; ok && i < min(count, L::kRaw); ++i) ok = fetch(i);
+            if (!ok) break;
             // the largest V scale of the keys in reach
             float v_top = 1e-30f;
             const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
@@ -796,82 +817,84 @@ __global__ void __launch_bounds__(kThreads, 1)
                     v_top = fmaxf(v_top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
             }
             v_top = warp_max(v_top);
-            // rows of Q, brought into f16's range by a power of two each: a warp to a row
+            // rows of Q, brought into f16's range by a power of two each: D / 8 lanes to a row,
+            // eight loads of a lane under way
             const uint32_t qb = units % kQBufs;
             if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
             int8_t* back = s_back + units % L::kBackSlots * 2 * kTileRows;
             if (i0 == 0) s_top[units % L::kBackSlots] = v_top;
             uint8_t* to_q = sQ + qb * 2 * L::kOperand;
             ++units;
-            for (uint32_t r0 = i0 / 32; r0 < w.tiles * kTileRows; r0 += 4 * kConverters) {
-                // a lane has D / 32 values of each of four rows
-                uint32_t q2[4][D / 64];
+            constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // of a row; rows of a load
+            const uint32_t chunk = lane % kLanes;
+#pragma unroll 1
+            for (uint32_t r0 = i0 / 32 * 8 * kRows; r0 < w.tiles * kTileRows; r0 += kConverters * 8 * kRows) {
+                uint4 x[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t row = w.row0 + r0 + kConverters * e;
-                    const bool live = r0 + kConverters * e < w.tiles * kTileRows && row < w.where.rows;
-                    const uint16_t* q = static_cast<const uint16_t*>(p.q) +
-                                        (live ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) : 0);
-#pragma unroll
-                    for (int k = 0; k < D / 64; ++k)
-                        q2[e][k] = live && D / 32 * lane + 2 * k < p.head_dim
-                                       ? *reinterpret_cast<const uint32_t*>(q + D / 32 * lane + 2 * k)
-                                       : 0u;
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint32_t r = r0 + k * kRows + lane / kLanes, row = w.row0 + r;
+                    x[k] = make_uint4(0, 0, 0, 0);
+                    if (r < w.tiles * kTileRows && row < w.where.rows && 8 * chunk < p.head_dim)
+                        x[k] = *reinterpret_cast<const uint4*>(
+                            static_cast<const uint16_t*>(p.q) +
+                            row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) + 8 * chunk);
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t r = r0 + kConverters * e;
-                    if (r >= w.tiles * kTileRows) break;
+                for (uint32_t k = 0; k < 8; ++k) {
+                    const uint32_t r = r0 + k * kRows + lane / kLanes;
+                    uint32_t* y = reinterpret_cast<uint32_t*>(&x[k]);
                     float most = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < D / 64; ++k) {
-                        const float2 y = unpack2(q2[e][k], p.q_bf16);
-                        most = fmax3(most, fabsf(y.x), fabsf(y.y));
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = unpack2(y[e], p.q_bf16);
+                        most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
                     }
-                    most = warp_max(most);
+#pragma unroll
+                    for (uint32_t o = kLanes / 2; o; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                     int ex = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
                     ex = max(-120, min(120, ex));
                     const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
-                    if (lane == 0) back[r] = (int8_t)ex;
 #pragma unroll
-                    for (int k = 0; k < D / 64; ++k) {
-                        const float2 y = unpack2(q2[e][k], p.q_bf16);
-                        const uint32_t dim = D / 32 * lane + 2 * k;
-                        *reinterpret_cast<uint32_t*>(to_q + (r / kTileRows) * L::kOperand +
-                                                     chunk_at(r % kTileRows, dim / 8) + 2 * (dim % 8)) =
-                            pack2<false>(y.x * up, y.y * up);
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 v = unpack2(y[e], p.q_bf16);
+                        y[e] = pack2<false>(v.x * up, v.y * up);
                     }
+                    if (r >= w.tiles * kTileRows) continue;
+                    if (chunk == 0) back[r] = (int8_t)ex;
+                    *reinterpret_cast<uint4*>(to_q + (r / kTileRows) * L::kOperand + chunk_at(r % kTileRows, chunk)) = x[k];
                 }
             }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[qb]);
-            auto convert = [&](uint32_t h, uint4 (&x)[kLoads]) -> bool {
-                const uint32_t at = ring + h / 2, st = at % kStages;
-                if (!(h & 1) && !warp_wait(&empty[st], (at / kStages) ^ 1u)) return false;
+            for (uint32_t i = 0; ok && i < count; ++i) {
+                const uint32_t at = ring + i, st = at % kStages, slot = at % L::kRaw;
+                ok = warp_wait(&raw_full[slot], at / L::kRaw) && warp_wait(&empty[st], (at / kStages) ^ 1u);
+                if (!ok) break;
                 uint8_t* to = sKV + st * L::kOperand;
+                const uint8_t* from = sRaw + slot * L::kRawBytes;
 #pragma unroll
-                for (uint32_t k = 0; k < kLoads; ++k) {
-                    const uint32_t at16 = i0 + kStep * k, in_half = at16 / kParts, part = at16 % kParts;
-                    const uint32_t key = in_half + (h & 1) * kHalf;
-                    if (in_half >= kHalf) continue;
-                    const uint32_t w4[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u,
-                                            x[k].w ^ 0x80808080u};
+                for (uint32_t k = 0; k < (kKeys * kParts + kStep - 1) / kStep; ++k) {
+                    const uint32_t at16 = i0 + kStep * k, key = at16 / kParts, part = at16 % kParts;
+                    if (key >= kKeys) continue;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (16 * part < p.head_dim) x = *reinterpret_cast<const uint4*>(from + key * p.head_dim + 16 * part);
+                    const uint32_t w4[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
                     *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part)) =
                         make_uint4(codes_lo(w4[0]), codes_hi(w4[0]), codes_lo(w4[1]), codes_hi(w4[1]));
                     *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part + 1)) =
                         make_uint4(codes_lo(w4[2]), codes_hi(w4[2]), codes_lo(w4[3]), codes_hi(w4[3]));
                 }
-                if (h & 1) {
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&full[st]);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&full[st]);
+                    mbar_arrive(&raw_empty[slot]);
                 }
-                if (h + 2 < 4 * w.blocks) load(h + 2, x);
-                return true;
-            };
-            for (uint32_t h = 0; ok && h < 4 * w.blocks; h += 2) ok = convert(h, x[0]) && convert(h + 1, x[1]);
-            ring += 2 * w.blocks;
+                __syncwarp();
+                if (i0 < 32 && i + L::kRaw < count) ok = fetch(i + L::kRaw);
+            }
+            ring += count;
         }
     }
 
@@ -934,7 +957,7 @@ bool encode_queries(CUtensorMap& tm, const RowsParams& p, uint32_t tokens, bool 
 template <int D, bool kS8, bool kBF16>
 int start(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, const TilesParams& n, uint32_t units,
           cudaStream_t st) {
-    using L = Layout<D>;
+    using L = Layout<D, kS8>;
     auto kernel = attention_tiles_kernel<D, kS8, kBF16>;
     static std::atomic<uint64_t> configured;  // one bit per device ordinal
     int dev = 0;
