@@ -20,9 +20,6 @@ struct Plan {
     uint64_t slots;      // row blocks over all sequences
 };
 
-#ifndef DAV2_TILES_FROM
-#define DAV2_TILES_FROM 33
-#endif
 // Rows that share a key head decide the kernel. Keys are split where the row blocks
 // alone would leave SMs idle, down to 128 keys (tiles kernel: 256) to a block.
 Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_length, uint32_t group,
@@ -32,23 +29,25 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_lengt
     const uint64_t each = ragged ? (queries + sequences - 1) / sequences : queries;
     const uint64_t rows = each * group;
     n.row_tiles = rows <= 8 ? 1 : 2;
-    n.row_warps = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-    if (rows >= DAV2_TILES_FROM) n.row_warps = 0;
+    n.row_warps = rows <= 16 ? 1 : 2;
+    // 32 and 64 rows of 64 dims over 2000 keys, rows and tiles kernel: 12.4 and 15.0, 19.5 and
+    // 16.0 us; 64 rows of 128 dims over 4000 tokens in the cache: 55 and 42 us
+    if (rows > 32) n.row_warps = 0;
     const uint64_t tile = n.row_warps ? 8ull * n.row_tiles * n.row_warps : 256;
     n.slots = ragged ? queries * group / tile + sequences : sequences * ((rows + tile - 1) / tile);
     const uint64_t live = std::max<uint64_t>(1, sequences * ((rows + tile - 1) / tile)) * kv_heads;
     n.clusters = false;
     if (!n.row_warps) {
         // the split count that ends first: rounds of units over the SMs, each a number of
-        // 128-key blocks (about 2 us) and about four more to begin and end; the parts are
-        // written and read at about 5 TB/s, and their join is a launch
+        // 128-key blocks (about 2 us) and as much as eight more to begin and end; the parts, written
+        // and read again, about 2 us for 5 MB, and the join a launch
         const uint64_t blocks = (max_length + 127ull) / 128;
         const uint64_t part = rows * sequences * kv_heads * (head_dim * 8ull + 16);
         uint64_t best = ~0ull;
         n.splits = 1;
         for (uint64_t s = 1; s <= 32 && s * 4 <= std::max<uint64_t>(blocks, 4); ++s) {
-            const uint64_t cost = (live * s + kSms - 1) / kSms * ((blocks + s - 1) / s + 4) +
-                                  (s > 1 ? 3 + s * part / 10000000 : 0);
+            const uint64_t cost = (live * s + kSms - 1) / kSms * ((blocks + s - 1) / s + 8) +
+                                  (s > 1 ? 3 + s * part / 5000000 : 0);
             if (cost < best) best = cost, n.splits = (uint32_t)s;
         }
         return n;

@@ -12,8 +12,8 @@
 // of O. While one tile's softmax runs, the tensor cores work on the other tile; at
 // D = 64 also S of the next block, as P has columns of its own.
 //
-// One block runs on an SM at a time and takes over the units of blocks that have not
-// started yet, one after the other (cluster launch control), so that units of different
+// One block runs on an SM at a time and, a little into its unit, takes over that of a
+// block that has not started yet (cluster launch control), so that units of different
 // lengths spread evenly; its roles run ahead of one another across units: Q and the first
 // keys of the next unit are loaded, and its first S computed, while the softmax warps
 // still write the last unit's rows.
@@ -87,6 +87,7 @@ static_assert(Layout<128, false>::kSmem <= 232448 && Layout<64, false>::kSmem <=
               "shared memory above the per-block limit");
 
 struct TilesParams {
+    uint32_t takes_over;  // more units than SMs
     uint32_t q_box;  // Q by TMA: tokens of a 128-row box (0: by a warp)
     uint32_t slots, full_units, full_tiles;  // full_*: dense batches
 };
@@ -321,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // The unit after the `iter`-th one of this block; false: there is none (or a timeout).
     auto next_unit = [&](uint32_t iter, uint32_t& u) -> bool {
+        if (!n.takes_over) return false;
         const uint32_t slot = iter & 1u;
         if (!warp_wait(&unit_full[slot], iter >> 1)) return false;
         const bool more = read_unit(&response[slot], u);
@@ -585,17 +587,24 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t u = blockIdx.x;
         for (uint32_t iter = 0;; ++iter) {
             if (iter && !next_unit(iter - 1, u)) break;
-            // ask for the next unit once every warp has read the response before the last
-            const uint32_t slot = iter & 1u;
-            if (role == 0 && !warp_wait(&unit_empty[slot], ((iter >> 1) & 1u) ^ 1u)) break;
-            if (role == 0 && lane == 0) {
+            // Asks for the next unit, once every warp has read the response before the last.
+            // Not at the beginning: a block that has not started may be about to, on an idle SM.
+            auto ask = [&]() -> bool {
+                if (!n.takes_over || role != 0) return true;
+                const uint32_t slot = iter & 1u;
+                if (!wait(&unit_empty[slot], ((iter >> 1) & 1u) ^ 1u)) return false;
                 fence_async_smem();
                 mbar_arrive_expect_tx(&unit_full[slot], 16);
                 request_unit(&response[slot], &unit_full[slot]);
-            }
-            __syncwarp();
+                return true;
+            };
             const Unit w = unit_at(p, n, u);
-            if (!w.blocks) continue;
+            if (!w.blocks) {
+                bool ok = true;
+                if (lane == 0) ok = ask();
+                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+                continue;
+            }
             const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
             const uint32_t tiles = w.tiles, blocks = w.blocks;
             const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
@@ -625,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t j = 0; ok && j < blocks; ++j) {
                     const bool more = j + 1 < blocks;
                     const uint32_t sv = stage;
-                    ok = wait(&full[sv], phase);
+                    if (j == min(2u, blocks - 1)) ok = ask();
+                    ok = ok && wait(&full[sv], phase);
                     next_stage(1);
                     const uint32_t sk = stage;
                     if (more) {
@@ -1000,6 +1010,9 @@ int launch_attention_tiles(const RowsParams& p, uint32_t slots, bool s8, bool bf
                                          : full_units + (rows % (2 * kTileRows) ? heads * p.sequences : 0);
     if (units > 0x7FFFFFFFu) return set_error(DAV2CUDA_INVALID_ARGUMENT, "attention: too many row tiles");
     n.full_units = (uint32_t)full_units;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    n.takes_over = units > (uint64_t)sm_count(dev);
     const bool small = p.head_dim <= 64;
     if (s8) return small ? start<64, true, false>(q, k, v, p, n, (uint32_t)units, st) : start<128, true, false>(q, k, v, p, n, (uint32_t)units, st);
     if (bf16) return small ? start<64, false, true>(q, k, v, p, n, (uint32_t)units, st) : start<128, false, true>(q, k, v, p, n, (uint32_t)units, st);
