@@ -12,7 +12,7 @@
 // of O. While one tile's softmax runs, the tensor cores work on the other tile; at
 // D = 64 also S of the next block, as P has columns of its own.
 //
-// One block runs on an SM at a time and, a little into its unit, takes over that of a
+// One block runs on an SM at a time and takes over, unit after unit, that of a
 // block that has not started yet (cluster launch control), so that units of different
 // lengths spread evenly; its roles run ahead of one another across units: Q and the first
 // keys of the next unit are loaded, and its first S computed, while the softmax warps
@@ -330,6 +330,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&unit_empty[slot]);
         return more;
     };
+    // Asks for it (one thread), once every warp has read the response before the last. Not
+    // at a unit's beginning: a block that has not started may be about to, on an idle SM.
+    auto ask = [&](uint32_t iter) -> bool {
+        if (!n.takes_over) return true;
+        const uint32_t slot = iter & 1u;
+        if (!mbar_wait(&unit_empty[slot], ((iter >> 1) & 1u) ^ 1u, abort_flag, p.err)) return false;
+        fence_async_smem();
+        mbar_arrive_expect_tx(&unit_full[slot], 16);
+        request_unit(&response[slot], &unit_full[slot]);
+        return true;
+    };
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax
@@ -369,6 +380,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 c *= __uint_as_float((uint32_t)(127 - s_back[unit % L::kBackSlots * 2 * kTileRows + t * kTileRows + r]) << 23);
                 v_top = s_top[unit % L::kBackSlots];
             }
+            // where the row's result goes, found now: the unit's numbers need no registers later
+            const uint64_t at = !live ? 0
+                                : p.splits > 1 ? part_at(p, w.where, w.kv_head, row, w.split)
+                                               : row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
             const uint32_t reach = reach_of(p, w.where, w.len, row);
             const uint32_t low = __reduce_min_sync(0xffffffffu, live ? reach : 0xFFFFFFFFu);
             // codes: lane i has the K scale (i < 8), lane 8 + i the V scale over the largest,
@@ -428,15 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 128; ++i)
                         if (key0 + i >= reach) s[i] = -INFINITY;
                 }
-                float a[43];
+                // four chains: a tree's partial maxima beside 128 scores would not fit the registers
+                float a[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 0; i < 42; ++i) a[i] = fmax3(s[3 * i], s[3 * i + 1], s[3 * i + 2]);
-                a[42] = fmax3(s[126], s[127], s[127]);
+                for (int i = 4; i < 124; i += 8)
 #pragma unroll
-                for (int i = 0; i < 14; ++i) a[i] = fmax3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = fmax3(a[3 * i], a[3 * i + 1], a[3 * i + 2]);
-                float top = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[12], a[13]), a[42]);
+                    for (int e = 0; e < 4; ++e) a[e] = fmax3(a[e], s[i + 2 * e], s[i + 2 * e + 1]);
+                a[0] = fmax3(a[0], s[124], s[125]), a[1] = fmax3(a[1], s[126], s[127]);
+                float top = fmax3(fmax3(a[0], a[1], a[2]), a[3], a[3]);
                 if constexpr (!kS8) top = top == -INFINITY ? top : top * c;
                 if constexpr (!L::kAlias) {
                     // P's columns, and O: the product of the block before is done
@@ -501,9 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float unit_v = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
             const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
             const float f = l != 0.0f ? (p.splits == 1 ? unit_v / l : unit_v * back) : 0.0f;
-            const uint64_t slot = live && p.splits > 1 ? part_at(p, w.where, w.kv_head, row, w.split) : 0;
-            const uint64_t at = live ? row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride) : 0;
-            if (live && p.splits > 1) p.part_ml[slot] = make_float2(m, l * back);
+            if (live && p.splits > 1) p.part_ml[at] = make_float2(m, l * back);
 #pragma unroll 1
             for (uint32_t k = 0; k < D / 32; ++k) {
                 uint32_t o[32];
@@ -517,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = l != 0.0f ? __uint_as_float(o[i + e]) * f : 0.0f;
                     if (p.splits > 1 || p.out_kind == 0) {
-                        float* to = p.splits > 1 ? p.part_o + slot * p.head_dim : static_cast<float*>(p.out) + at;
+                        float* to = p.splits > 1 ? p.part_o + at * p.head_dim : static_cast<float*>(p.out) + at;
                         float4* to4 = reinterpret_cast<float4*>(to + 32 * k + i);
                         to4[0] = make_float4(x[0], x[1], x[2], x[3]);
                         to4[1] = make_float4(x[4], x[5], x[6], x[7]);
@@ -535,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();  // O is read: the next unit's first product, after its P, may overwrite it
         }
     } else if (warp < kSoftmaxWarps + kIssuers<D, kS8>) {
-        // ------------------------------------------- products, and the next unit
+        // ----------------------------------------------------------- products
         // One thread issues, with everything but the waits unrolled: between its products the
         // tensor cores may wait, as their queue holds a few (rolled up, 5 to 15% slower).
         constexpr uint32_t ab = kBF16 ? 1u : 0u;
@@ -587,24 +599,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t u = blockIdx.x;
         for (uint32_t iter = 0;; ++iter) {
             if (iter && !next_unit(iter - 1, u)) break;
-            // Asks for the next unit, once every warp has read the response before the last.
-            // Not at the beginning: a block that has not started may be about to, on an idle SM.
-            auto ask = [&]() -> bool {
-                if (!n.takes_over || role != 0) return true;
-                const uint32_t slot = iter & 1u;
-                if (!wait(&unit_empty[slot], ((iter >> 1) & 1u) ^ 1u)) return false;
-                fence_async_smem();
-                mbar_arrive_expect_tx(&unit_full[slot], 16);
-                request_unit(&response[slot], &unit_full[slot]);
-                return true;
-            };
             const Unit w = unit_at(p, n, u);
-            if (!w.blocks) {
-                bool ok = true;
-                if (lane == 0) ok = ask();
-                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-                continue;
-            }
+            if (!w.blocks) continue;
             const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
             const uint32_t tiles = w.tiles, blocks = w.blocks;
             const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
@@ -634,8 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t j = 0; ok && j < blocks; ++j) {
                     const bool more = j + 1 < blocks;
                     const uint32_t sv = stage;
-                    if (j == min(2u, blocks - 1)) ok = ask();
-                    ok = ok && wait(&full[sv], phase);
+                    ok = wait(&full[sv], phase);
                     next_stage(1);
                     const uint32_t sk = stage;
                     if (more) {
@@ -691,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if constexpr (!kS8) {
         uint32_t ring = 0, units = 0;
         if (warp == 10) {
-            // ------------------------------------------------------------ TMA
+            // -------------------------------------------------- TMA, and the next unit
             uint32_t u = blockIdx.x;
             for (uint32_t iter = 0;; ++iter) {
                 if (iter && !next_unit(iter - 1, u)) break;
@@ -699,9 +694,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = true;
                 if (lane == 0) {
                     const int k_batch = p.k_batch ? (int)w.where.seq : 0, v_batch = p.v_batch ? (int)w.where.seq : 0;
+                    if (!w.blocks) ok = ask(iter);
                     for (uint32_t i = 0; i < 2 * w.blocks; ++i) {
                         const uint32_t at = ring + i, st = at % kStages;
-                        if (*abort_flag || !mbar_wait(&empty[st], ((at / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+                        if (i == min(kStages + 1, 2 * w.blocks - 1)) ok = ask(iter);
+                        if (!ok || *abort_flag || !mbar_wait(&empty[st], ((at / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
                             ok = false;
                             break;
                         }
@@ -773,7 +770,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t iter = 0; ok; ++iter) {
             if (iter && !next_unit(iter - 1, u)) break;
             const Unit w = unit_at(p, n, u);
-            if (!w.blocks) continue;
+            if (!w.blocks) {
+                if (i0 == 0) ok = ask(iter);
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                continue;
+            }
             // lanes 0 to 7 have the page of their piece of a block, fetched a block ahead
             const uint32_t piece = min(1u << p.page_shift, kKeys);
             auto page_of = [&](uint32_t j) -> int32_t {
@@ -900,6 +901,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (lane == 0) {
                     mbar_arrive(&full[st]);
                     mbar_arrive(&raw_empty[slot]);
+                }
+                if (i == min(4u, count - 1)) {
+                    if (i0 == 0) ok = ask(iter);
+                    ok = __shfl_sync(0xffffffffu, ok, 0);
+                    if (!ok) break;
                 }
                 __syncwarp();
                 if (i0 < 32 && i + L::kRaw < count) ok = fetch(i + L::kRaw);
