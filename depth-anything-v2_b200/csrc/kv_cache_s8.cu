@@ -9,19 +9,19 @@
 // ratio rounded to f32. Infinities take the codes +-127 and NaN the code 0, and
 // neither enters a scale.
 //
-// Bound by memory: the rows are read from HBM once (the second pass over a
-// page's rows, at most 128 rows of one head, finds them in L1 or L2) and the codes
-// written once. One block for each page that receives tokens, each head, and K or
+// Bound by memory: the rows are read once, into registers, and the codes written once. One block for each page that receives tokens, each head, and K or
 // V; the blocks of sequence s are numbered from floor(begin[s] / page_tokens) + 2 s,
 // which leaves room for its pages whatever their boundaries, so that the host
 // needs no length: blocks without a page leave at once.
+#include <type_traits>
+
 #include "abi_check.h"
 #include "kernels.cuh"
 
 namespace dav2cuda {
 namespace {
 
-constexpr uint32_t kThreads = 128;
+constexpr uint32_t kMost = 8;  // vectors of eight values that a thread keeps in registers
 
 struct AppendParams {
     int8_t* codes[2];  // K, V
@@ -35,35 +35,59 @@ struct AppendParams {
     int* err;
 };
 
-// Eight consecutive values as f32; NaN as 0.
+// Eight consecutive values as they lie in memory.
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const T* p) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        union {
-            uint4 u;
-            T t[8];
-        } a;
-        a.u = *reinterpret_cast<const uint4*>(p);
+struct Vector {
+    uint4 u[sizeof(T) / 2];
+
+    __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(a.t[i]);
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
     }
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] == x[i] ? x[i] : 0.0f;
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+        const T* t = reinterpret_cast<const T*>(u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(t[i]);
+    }
+    // The largest magnitude's bits so far, 16-bit values two to a word: magnitudes order as
+    // their bits do, infinities and NaN above all others.
+    __device__ __forceinline__ uint32_t largest(uint32_t most) const {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+            const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) most = max(most, w[e] & 0x7FFFFFFFu);
+                else most = __vmaxu2(most, w[e] & 0x7FFF7FFFu);
+            }
+        }
+        return most;
+    }
+};
+
+// A magnitude from its bits.
+template <typename T>
+__device__ __forceinline__ float from_bits(uint32_t bits) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(bits);
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half((unsigned short)bits));
+    else return __uint_as_float(bits << 16);
 }
 
-template <typename T>
+template <typename T, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads) kv_cache_append_kernel(const AppendParams p) {
-    const uint32_t which = blockIdx.z, head = blockIdx.y;
+    // K and V of a token's heads lie side by side: neighbouring blocks read neighbouring bytes
+    const uint32_t slot = blockIdx.x / (2 * p.heads), which = blockIdx.x / p.heads % 2, head = blockIdx.x % p.heads;
     const uint32_t page_tokens = 1u << p.page_shift;
     // the last sequence whose blocks begin at or before this one
-    const uint32_t s = warp_last_at_most(p.sequences, blockIdx.x, [&](uint32_t i) {
+    const uint32_t s = warp_last_at_most(p.sequences, slot, [&](uint32_t i) {
         return (uint64_t)((uint32_t)p.begin[i] >> p.page_shift) + 2 * i;
     });
     const int64_t begin = p.begin[s], end = p.begin[s + 1], cached = p.cached[s];
-    const int64_t j = (int64_t)blockIdx.x - ((begin >> p.page_shift) + 2 * (int64_t)s);
+    const int64_t j = (int64_t)slot - ((begin >> p.page_shift) + 2 * (int64_t)s);
     if (j < 0) return;  // rows before the first sequence
     if (begin < 0 || end < begin || end > (int64_t)p.tokens || cached < 0) {
         if (threadIdx.x == 0 && head == 0) atomicExch(p.err, 3);
@@ -86,24 +110,53 @@ __global__ void __launch_bounds__(kThreads) kv_cache_append_kernel(const AppendP
     const uint64_t unit = (uint64_t)page * p.heads + head;
     int8_t* codes = p.codes[which] + ((unit << p.page_shift) * p.head_dim);
 
-    float most = 0.0f;
-    for (uint32_t i = threadIdx.x; i < count * per_row; i += kThreads) {
-        const uint32_t row = i / per_row, col = i - row * per_row;
-        float x[8];
-        load8(x, rows + row * p.stride[which] + col * 8);
+    // The rows of the page: in registers where a thread has at most kMost vectors of them,
+    // all loads under way at once; else (a short block's long page) read again below.
+    const uint32_t vectors = count * per_row;
+    const uint32_t inverse_row = (65535 + per_row) / per_row;  // i / per_row of i < 65536 / 16
+    const bool once = vectors <= kThreads * kMost;
+    auto at = [&](uint32_t i) -> const T* {
+        const uint32_t row = (i * inverse_row) >> 16;
+        return rows + row * p.stride[which] + (i - row * per_row) * 8;
+    };
+    Vector<T> x[kMost];
+    uint32_t bits = 0;
+    for (uint32_t base = threadIdx.x; base < vectors; base += kThreads * kMost) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float a = fabsf(x[e]);
-            most = fmaxf(most, a < INFINITY ? a : 0.0f);
+        for (uint32_t k = 0; k < kMost; ++k) {
+            const uint32_t i = base + k * kThreads;
+            if (i < vectors) x[k].load(at(i));
+            else x[k].clear();
         }
+#pragma unroll
+        for (uint32_t k = 0; k < kMost; ++k) bits = x[k].largest(bits);
     }
-    __shared__ float s_most[kThreads / 32];
-    most = warp_max(most);
-    if ((threadIdx.x & 31) == 0) s_most[threadIdx.x / 32] = most;
+    if constexpr (sizeof(T) == 2) bits = max(bits & 0xFFFFu, bits >> 16);
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    __shared__ uint32_t s_bits[kThreads / 32];
+    if ((threadIdx.x & 31) == 0) s_bits[threadIdx.x / 32] = bits;
     const float old = held ? p.scales[which][unit] : 0.0f;
     __syncthreads();
 #pragma unroll
-    for (uint32_t w = 0; w < kThreads / 32; ++w) most = fmaxf(most, s_most[w]);
+    for (uint32_t w = 0; w < kThreads / 32; ++w) bits = max(bits, s_bits[w]);
+    float most = from_bits<T>(bits);
+    const bool odd = !(most < INFINITY);  // an infinity or NaN: the largest finite magnitude, the long way
+    if (odd) {
+        most = 0.0f;
+        for (uint32_t i = threadIdx.x; i < vectors; i += kThreads) {
+            Vector<T> y;
+            y.load(at(i));
+            float f[8];
+            y.floats(f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(f[e]) < INFINITY ? fabsf(f[e]) : 0.0f);
+        }
+        most = warp_max(most);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) s_bits[threadIdx.x / 32] = __float_as_uint(most);
+        __syncthreads();
+        for (uint32_t w = 0; w < kThreads / 32; ++w) most = fmaxf(most, __uint_as_float(s_bits[w]));
+    }
     const float need = fmaxf(__fdiv_rn(most, 127.0f), 1e-8f);
     const bool grows = held == 0 || need > old;
     const float scale = grows ? need : old;
@@ -119,15 +172,31 @@ __global__ void __launch_bounds__(kThreads) kv_cache_append_kernel(const AppendP
     }
     const float inverse = __frcp_rn(scale);
     uint2* to = reinterpret_cast<uint2*>(codes + (uint64_t)held * p.head_dim);
-    for (uint32_t i = threadIdx.x; i < count * per_row; i += kThreads) {
-        const uint32_t row = i / per_row, col = i - row * per_row;
-        float x[8];
-        load8(x, rows + row * p.stride[which] + col * 8);
-        to[i] = make_uint2(q8x4_quot(x[0], x[1], x[2], x[3], scale, inverse),
-                           q8x4_quot(x[4], x[5], x[6], x[7], scale, inverse));
+    for (uint32_t base = threadIdx.x; base < vectors; base += kThreads * kMost) {
+#pragma unroll
+        for (uint32_t k = 0; k < kMost; ++k) {
+            const uint32_t i = base + k * kThreads;
+            if (i >= vectors) break;
+            if (!once) x[k].load(at(i));
+            float f[8];
+            x[k].floats(f);
+            if (odd) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = f[e] == f[e] ? f[e] : 0.0f;
+            }
+            to[i] = make_uint2(q8x4_quot(f[0], f[1], f[2], f[3], scale, inverse),
+                               q8x4_quot(f[4], f[5], f[6], f[7], scale, inverse));
+        }
     }
     __syncthreads();  // every thread has read the old scale
     if (grows && threadIdx.x == 0) p.scales[which][unit] = scale;
+}
+
+template <uint32_t kThreads>
+void start(const AppendParams& p, uint32_t blocks, uint32_t precision, cudaStream_t st) {
+    if (precision == 0) kv_cache_append_kernel<float, kThreads><<<blocks, kThreads, 0, st>>>(p);
+    else if (precision == 1) kv_cache_append_kernel<__nv_bfloat16, kThreads><<<blocks, kThreads, 0, st>>>(p);
+    else kv_cache_append_kernel<__half, kThreads><<<blocks, kThreads, 0, st>>>(p);
 }
 
 }  // namespace
@@ -145,7 +214,7 @@ extern "C" DAV2CUDA_API int dav2cuda_kv_cache_append_s8(
                  "cache append: head_dim must be a multiple of 16, 16 to 128");
     DAV2_REQUIRE(page_tokens >= 16 && page_tokens <= 128 && (page_tokens & (page_tokens - 1)) == 0,
                  "cache append: page_tokens must be 16, 32, 64 or 128");
-    DAV2_REQUIRE(kv_heads >= 1 && kv_heads <= 65535 && page_count >= 1 && page_count <= 0x7FFFFFFFu && table_stride >= 1,
+    DAV2_REQUIRE(kv_heads >= 1 && kv_heads <= 32767 && page_count >= 1 && page_count <= 0x7FFFFFFFu && table_stride >= 1,
                  "invalid cache append dimensions");
     DAV2_REQUIRE(tokens <= 0x7FFFFFFFu && sequences <= 0x1FFFFFFFu, "cache append: too many tokens or sequences");
     if (tokens == 0 || sequences == 0) return DAV2CUDA_OK;
@@ -170,10 +239,12 @@ extern "C" DAV2CUDA_API int dav2cuda_kv_cache_append_s8(
     p.table_stride = table_stride;
     p.err = device_error_word();
     if (!p.err) return set_error(DAV2CUDA_INTERNAL_ERROR, "cache append: no device error word");
-    const dim3 grid((tokens >> p.page_shift) + 2 * sequences, kv_heads, 2);
+    const uint64_t blocks = ((uint64_t)(tokens >> p.page_shift) + 2ull * sequences) * kv_heads * 2;
+    DAV2_REQUIRE(blocks <= 0x7FFFFFFFu, "cache append: too many tokens or sequences");
     const cudaStream_t st = as_stream(stream);
-    if (precision == 0) kv_cache_append_kernel<float><<<grid, kThreads, 0, st>>>(p);
-    else if (precision == 1) kv_cache_append_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(p);
-    else kv_cache_append_kernel<__half><<<grid, kThreads, 0, st>>>(p);
+    // a few tokens for each sequence are the work of few threads, and blocks of few threads all
+    // fit the SMs at once (64 sequences, one token each: STEP us)
+    if (tokens <= 4ull * sequences) start<64>(p, (uint32_t)blocks, precision, st);
+    else start<128>(p, (uint32_t)blocks, precision, st);
     return check_launch("kv_cache_append_s8");
 }

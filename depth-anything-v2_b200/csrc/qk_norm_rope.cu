@@ -29,7 +29,7 @@ namespace {
 
 constexpr uint32_t kMaxHead = 256;
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxTokens = 4;  // tokens of one block
+constexpr uint32_t kMaxTokens = 8;  // tokens of one block
 
 struct RopeParams {
     void* out[2];  // q, k
@@ -332,10 +332,10 @@ extern "C" DAV2CUDA_API int dav2cuda_qk_norm_rope(
     cudaGetDevice(&dev);
     const uint32_t sms = (uint32_t)sm_count(dev);
     if (!sms) return set_error(DAV2CUDA_LAUNCH_FAILED, "qk norm rope: cannot query the SM count");
-    // Four tokens to a block, so that a block's angles serve many rows; one token,
+    // Eight tokens to a block, so that a block's angles serve many rows; one token,
     // and its heads over several blocks, where that would leave SMs idle.
     const uint32_t heads = q_heads + k_heads;
-    p.block_tokens = tokens >= 8 * sms ? kMaxTokens : 1;
+    p.block_tokens = tokens >= 16 * sms ? kMaxTokens : 1;
     uint32_t lanes = 32;
     if (vectors)
         for (lanes = 1; lanes < head_dim / 16;) lanes *= 2;
