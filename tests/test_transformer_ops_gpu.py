@@ -388,6 +388,103 @@ def test_attention_scale_zero_and_negative(cuda, dav2lib, scale, queries):
     assert ref.outside(out, want, bound) <= 1
 
 
+@pytest.mark.parametrize("p", [1, 2])
+@pytest.mark.parametrize("hq,hkv,d", [(16, 16, 64), (8, 2, 128), (12, 4, 64), (6, 2, 128)])
+def test_cross_attention_more_units_than_sms(cuda, dav2lib, hq, hkv, d, p):
+    """Several units of work to an SM, some without keys, some of one row tile; groups that divide a tile and groups
+    that do not."""
+    batch = 40
+    lengths = [(i * 53) % 334 if i % 5 else 0 for i in range(batch)]
+    check_cross(dav2lib, batch, 300, 333, hq, hkv, d, lengths, p, p, seed=hq)
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,causal", [(8, 8, 64, 16, True), (16, 4, 128, 128, True), (12, 4, 96, 64, False)])
+def test_cache_attention_more_units_than_sms(cuda, dav2lib, hq, hkv, d, page, causal):
+    n = 45
+    counts = [(i * 17) % 160 for i in range(n)]
+    lengths = [max(0, c + (i * 31) % 300 - 20) if i % 6 else 0 for i, c in enumerate(counts)]
+    check_cache(dav2lib, page, d, hq, hkv, lengths, counts, causal, 2, 2, seed=n)
+
+
+@pytest.mark.parametrize("queries", [2, 260])
+def test_cross_attention_shared_states_and_queries(cuda, dav2lib, queries):
+    """Batch strides of 0: one encoder's states for every batch entry, one set of queries for several encoders."""
+    g = gen(16)
+    q, k, v = (randn(g, 3, n, h, 64, dtype=torch.bfloat16) for n, h in ((queries, 4), (150, 2), (150, 2)))
+    out, lengths = torch.empty(3, queries, 4, 64, device="cuda"), ints([150, 20, 0])
+    for qq, kk, vv in ((q, k[:1].expand(3, -1, -1, -1), v[1:2].expand(3, -1, -1, -1)),
+                       (q[:1].expand(3, -1, -1, -1), k, v)):
+        cross(dav2lib, qq, kk, vv, lengths, 0.125, out)
+        done(dav2lib)
+        want, bound = ref.cross_attention(qq, kk, vv, [150, 20, 0], 0.125, 1, 0)
+        assert ref.outside(out, want, bound) <= 1
+
+
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cross_attention_nan_stays_where_it_is(cuda, dav2lib, queries, d):
+    """A NaN that a row sees makes that row NaN, and no other."""
+    g = gen(17)
+    q, k, v = (randn(g, 2, n, 2, d, dtype=torch.float16) for n in (queries, 200, 200))
+    for key in range(0, 130, 13):
+        kk = k.clone()
+        kk[1, key, 1, 5] = math.nan
+        out = torch.empty(2, queries, 2, d, device="cuda")
+        cross(dav2lib, q, kk, v, None, 0.125, out)
+        done(dav2lib)
+        assert out[1, :, 1].isnan().all()
+        want, bound = ref.cross_attention(q, k, v, [200, 200], 0.125, 2, 0)
+        keep = torch.ones_like(out, dtype=torch.bool)
+        keep[1, :, 1] = False
+        assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
+
+
+def test_attention_in_captured_graphs(cuda, dav2lib):
+    """Large calls captured into two graphs that share a workspace, replayed in turn on a side stream with new inputs."""
+    g = gen(18)
+    c = Cache(g, [900, 300, 0], 2, 128, 32)
+    lengths, counts = [900, 300, 0], [200, 100, 40]
+    begin = [0, 200, 300, 340]
+    lengths_d, begin_d = ints(lengths), ints(begin)
+    q = randn(g, 340, 8, 128, dtype=torch.float16)
+    x, k, v = randn(g, 2, 700, 4, 64, dtype=torch.float16), randn(g, 2, 800, 4, 64, dtype=torch.float16), randn(g, 2, 800, 4, 64, dtype=torch.float16)
+    o1, o2 = torch.empty(340, 8, 128, device="cuda"), torch.empty(2, 700, 4, 64, device="cuda")
+    args = (3, 340, 900, 8, 2, 128)
+    size = max(16, dav2lib.dav2cuda_attention_cache_s8_workspace_size(*args),
+               dav2lib.dav2cuda_cross_attention_16_workspace_size(2, 700, 800, 4, 4, 64))
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+
+    def first():
+        ok(dav2lib, dav2lib.dav2cuda_attention_cache_s8(
+            ptr(o1), ptr(q), ptr(c.k), ptr(c.ks), ptr(c.v), ptr(c.vs), ptr(c.table_d), ptr(lengths_d), ptr(begin_d), *args,
+            c.pages, c.page, c.table_d.shape[1], 1024, 1024, 0.1, 1, 2, 0, ptr(ws), size, stream()))
+
+    def second():
+        cross(dav2lib, x, k, v, None, 0.125, o2, ws)
+
+    side, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for call in (first, second):
+            call()  # sets the kernels up
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                call()
+            graphs.append(graph)
+        for _ in range(3):
+            q.copy_(randn(g, 340, 8, 128, dtype=torch.float16))
+            x.copy_(randn(g, 2, 700, 4, 64, dtype=torch.float16))
+            for graph in graphs:
+                graph.replay()
+            side.synchronize()
+            want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, lengths, begin, 0.1, True, 0)
+            assert ref.outside(o1, want, bound) <= 1
+            want, bound = ref.cross_attention(x, k, v, [800, 800], 0.125, 2, 0)
+            assert ref.outside(o2, want, bound) <= 1
+    done(dav2lib)
+
+
 def test_cross_attention_rows_in_any_order(cuda, dav2lib):
     """Batch and token strides of slices, q as a part of packed rows, k and v from different tensors."""
     g = gen(2)

@@ -82,8 +82,9 @@ def attend(q, k, v, scale, reach, p_unit, out_precision):
     """q [n, heads, d], k, v [tokens, heads, d] in 64 bits (heads alike), reach [n]: (o [n, heads, d], bound).
 
     Bound: p is rounded once (p_unit) and, held times 2^7 in f16, to no finer than 2^-32; a score is off by at most the
-    f32 sum's d roundings of sum |q||k|, which changes p by that relative amount, above and below the bar; ex2.approx,
-    the maximum's and the merges' factors add 2^-20; the result is rounded once."""
+    f32 sum's d roundings of sum |q||k|, which changes p by that relative amount, above and below the bar; an
+    exponential is off by 2^-22 (ex2.approx) or 2.7e-6 < 2^-18.4 (the polynomial), and the maximum's and the merges'
+    factors by a few 2^-22: together below 2^-18; the result is rounded once."""
     n, d = q.shape[0], q.shape[2]
     score = torch.einsum("nhd,thd->hnt", q, k) * scale
     size = torch.einsum("nhd,thd->hnt", q.abs(), k.abs()).amax() * abs(scale) if k.shape[0] else torch.zeros(())
@@ -93,7 +94,7 @@ def attend(q, k, v, scale, reach, p_unit, out_precision):
     o = torch.einsum("hnt,thd->nhd", p, v)
     spread = torch.einsum("hnt,thd->nhd", p, v.abs())
     least = 2.0 ** -32 * k.shape[0] * (v.abs().amax() if k.shape[0] else 0)
-    bound = (p_unit + 2 * (d + 8) * 2.0 ** -23 * float(size) + 2.0 ** -20) * spread + U[out_precision] * o.abs() + least
+    bound = (p_unit + 2 * (d + 8) * 2.0 ** -23 * float(size) + 2.0 ** -18) * spread + U[out_precision] * o.abs() + least
     return o, bound
 
 
