@@ -758,9 +758,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         // -------------------------------------------------------------- codes
-        // Warp 9 keeps kRaw tiles of codes under way from the pages (a page's tokens of a head
-        // are one run of bytes, copied in one piece); the three warps turn each into a 16-bit
-        // tile, 16 dims of a key at a time.
+        // kRaw tiles of codes are under way from the pages (a page's tokens of a head are one
+        // run of bytes, copied in one piece; the three warps start the copies in turn); the
+        // warps turn each into a 16-bit tile, 16 dims of a key at a time.
         constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
         const uint32_t i0 = threadIdx.x - 9 * 32;
         const uint32_t in_page = (1u << p.page_shift) - 1;
@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 continue;
             }
-            // lanes 0 to 7 have the page of their piece of a block, fetched a block ahead
+            // lanes 0 to 7 have the page of their piece of a block
             const uint32_t piece = min(1u << p.page_shift, kKeys);
             auto page_of = [&](uint32_t j) -> int32_t {
                 const uint32_t in_block = lane * piece, key = (w.first + j) * kKeys + in_block;
@@ -787,16 +787,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 return page;
             };
-            int32_t page_now = -1, page_next = i0 < 32 ? page_of(0) : -1;
+            const uint32_t count = 2 * w.blocks, turn_of = i0 / 32;
+            int32_t page_next = turn_of < count ? page_of(turn_of / 2) : -1;  // for the warp's next tile
             // Starts the copies of tile i (K_j: 2j, V_j: 2j + 1). Keys of no page, and past the
             // end, keep what the slot holds: any byte is a finite code, and they weigh nothing.
             auto fetch = [&](uint32_t i) -> bool {
                 const uint32_t at = ring + i, slot = at % L::kRaw;
                 if (!warp_wait(&raw_empty[slot], (at / L::kRaw) ^ 1u)) return false;
-                if (!(i & 1)) {
-                    page_now = page_next;
-                    if (i / 2 + 1 < w.blocks) page_next = page_of(i / 2 + 1);
-                }
+                const int32_t page_now = page_next;
+                if (i + kConverters < count) page_next = page_of((i + kConverters) / 2);
                 const uint32_t bytes = piece * p.head_dim;
                 const uint32_t live = __popc(__ballot_sync(0xffffffffu, page_now >= 0));
                 if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], live * bytes);
@@ -815,9 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 return true;
             };
-            const uint32_t count = 2 * w.blocks;
-            if (i0 < 32)
-                for (uint32_t i = 0; ok && i < min(count, L::kRaw); ++i) ok = fetch(i);
+            for (uint32_t i = turn_of; ok && i < min(count, L::kRaw); i += kConverters) ok = fetch(i);
             if (!ok) break;
             // the largest V scale of the keys in reach
             float v_top = 1e-30f;
@@ -886,7 +883,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint8_t* from = sRaw + slot * L::kRawBytes;
 #pragma unroll
                 for (uint32_t k = 0; k < (kKeys * kParts + kStep - 1) / kStep; ++k) {
-                    const uint32_t at16 = i0 + kStep * k, key = at16 / kParts, part = at16 % kParts;
+                    // eight lanes: four dims' parts of two rows, at D = 128 the first half of one and
+                    // the second of the other, which spreads loads and stores over the banks
+                    const uint32_t at16 = i0 + kStep * k;
+                    const uint32_t key = D == 64 ? at16 / 4 : at16 / 16 * 2 + (at16 / 4 & 1);
+                    const uint32_t part = D == 64 ? at16 % 4 : at16 % 4 + 4 * ((at16 / 4 ^ at16 / 8) & 1);
                     if (key >= kKeys) continue;
                     uint4 x = make_uint4(0, 0, 0, 0);
                     if (16 * part < p.head_dim) x = *reinterpret_cast<const uint4*>(from + key * p.head_dim + 16 * part);
@@ -908,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!ok) break;
                 }
                 __syncwarp();
-                if (i0 < 32 && i + L::kRaw < count) ok = fetch(i + L::kRaw);
+                if (i + L::kRaw < count && (i + L::kRaw) % kConverters == turn_of) ok = fetch(i + L::kRaw);
             }
             ring += count;
         }
