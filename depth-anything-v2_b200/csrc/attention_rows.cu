@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             x[1] += a * b.y;
         }
         if (p.splits == 1) {
-            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
             x[0] *= inv, x[1] *= inv;
             store_out(p, row_at(p, where, kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
         } else if (p.clusters) {
@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
         } else {
             const uint64_t slot = part_at(p, where, kv_head, row, blockIdx.z);
             if (dim == 0) p.part_ml[slot] = make_float2(top, sum);
-            if (sum > 0.0f) *reinterpret_cast<float2*>(p.part_o + slot * d + dim) = make_float2(x[0], x[1]);
+            if (sum != 0.0f) *reinterpret_cast<float2*>(p.part_o + slot * d + dim) = make_float2(x[0], x[1]);
         }
     }
     if (!p.clusters) return;
@@ -548,63 +548,80 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             x[0] += a * b.x;
             x[1] += a * b.y;
         }
-        const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
         x[0] *= inv, x[1] *= inv;
         store_out(p, row_at(p, where, kv_head, row, p.out_batch, p.out_stride) + dim, x, 2);
     }
     cluster_sync();  // no block leaves while another reads its shared memory
 }
 
-// Joins the splits of a row: each warp every fourth split, four dims to a lane, then
-// the warps' sums. Launched while the rows kernel still runs; waits for its end.
-__global__ void __launch_bounds__(kThreads) attention_join_kernel(const RowsParams p) {
-    __shared__ float s_f[kMaxSplits];
-    __shared__ float4 s_x[kWarps][32];
+// Joins the splits of a row, four dims to a lane: a warp to a row or (kWide, many splits)
+// a block, each warp every fourth split and then the warps' sums. Launched while the
+// kernel of the splits still runs; waits for its end.
+template <bool kWide>
+__global__ void __launch_bounds__(kThreads) attention_join_kernel(const RowsParams p, const uint64_t rows) {
+    __shared__ float s_f[kWide ? kMaxSplits : 1];
+    __shared__ float4 s_x[kWide ? kWarps : 1][32];
+    constexpr uint32_t kLoads = kWide ? kMaxSplits / 32 : 1;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t row = blockIdx.x;
+    const uint64_t row = kWide ? (uint64_t)blockIdx.x : (uint64_t)blockIdx.x * kWarps + warp;
     const uint32_t heads = p.kv_heads * p.group;
     const uint64_t token = row / heads;
     const uint32_t head = (uint32_t)(row - token * heads);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // rows of no sequence stay as they were
-    if (p.query_begin && ((int64_t)token < p.query_begin[0] || (int64_t)token >= p.query_begin[p.sequences])) return;
-    float top = kLowest, sum = 0.0f;
-    float2 ml[kMaxSplits / 32];
+    if (row >= rows || (p.query_begin && ((int64_t)token < p.query_begin[0] || (int64_t)token >= p.query_begin[p.sequences])))
+        return;
+    float top = kLowest, sum = 0.0f, weight = 0.0f;
+    float2 ml[kLoads];
 #pragma unroll
-    for (uint32_t i = 0; i < kMaxSplits / 32; ++i) {
+    for (uint32_t i = 0; i < kLoads; ++i) {
         const uint32_t k = 32 * i + lane;
         ml[i] = k < p.splits ? p.part_ml[row * p.splits + k] : make_float2(kLowest, 0.0f);
         top = fmaxf(top, ml[i].x);
     }
     top = warp_max(top);
 #pragma unroll
-    for (uint32_t i = 0; i < kMaxSplits / 32; ++i) {
-        const float f = ml[i].y > 0.0f ? ex2_approx(ml[i].x - top) : 0.0f;
-        sum += f * ml[i].y;
-        if (warp == 0) s_f[32 * i + lane] = f;
+    for (uint32_t i = 0; i < kLoads; ++i) {
+        // a split with no key in reach has written no sums
+        weight = ml[i].y != 0.0f ? ex2_approx(ml[i].x - top) : 0.0f;
+        sum += weight * ml[i].y;
+        if (kWide && warp == 0) s_f[32 * i + lane] = weight;
     }
     sum = warp_sum(sum);
-    __syncthreads();
     const uint32_t dim = 4 * lane;
+    const float* from = p.part_o + row * p.splits * p.head_dim + dim;
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (dim < p.head_dim) {
+    if constexpr (kWide) {
+        __syncthreads();
+        if (dim < p.head_dim) {
 #pragma unroll 8
-        for (uint32_t k = warp; k < p.splits; k += kWarps) {
-            const float f = s_f[k];
-            if (f == 0.0f) continue;  // no key of the split in reach: nothing was written
-            const float4 o = *reinterpret_cast<const float4*>(p.part_o + (row * p.splits + k) * p.head_dim + dim);
+            for (uint32_t k = warp; k < p.splits; k += kWarps) {
+                const float f = s_f[k];
+                if (f == 0.0f) continue;
+                const float4 o = *reinterpret_cast<const float4*>(from + (uint64_t)k * p.head_dim);
+                x.x += f * o.x, x.y += f * o.y, x.z += f * o.z, x.w += f * o.w;
+            }
+        }
+        s_x[warp][lane] = x;
+        __syncthreads();
+        if (warp) return;
+#pragma unroll
+        for (uint32_t w = 1; w < kWarps; ++w) {
+            const float4 y = s_x[w][lane];
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+    } else {
+#pragma unroll 8
+        for (uint32_t k = 0; k < p.splits; ++k) {
+            const float f = __shfl_sync(0xffffffffu, weight, k);
+            if (f == 0.0f || dim >= p.head_dim) continue;
+            const float4 o = *reinterpret_cast<const float4*>(from + (uint64_t)k * p.head_dim);
             x.x += f * o.x, x.y += f * o.y, x.z += f * o.z, x.w += f * o.w;
         }
     }
-    s_x[warp][lane] = x;
-    __syncthreads();
-    if (warp || dim >= p.head_dim) return;
-#pragma unroll
-    for (uint32_t w = 1; w < kWarps; ++w) {
-        const float4 y = s_x[w][lane];
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    if (dim >= p.head_dim) return;
+    const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
     const float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
     const uint64_t batch = p.query_begin ? 0 : token / p.queries;
     const uint64_t at = p.query_begin ? token * p.out_stride
@@ -665,12 +682,13 @@ int launch_attention_join(const RowsParams& p, uint64_t rows, cudaStream_t st) {
     early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((uint32_t)rows);
+    const bool wide = p.splits > 32;
+    config.gridDim = dim3((uint32_t)(wide ? rows : (rows + kWarps - 1) / kWarps));
     config.blockDim = dim3(kThreads);
     config.stream = st;
     config.attrs = early;
     config.numAttrs = 1;
-    cudaLaunchKernelEx(&config, attention_join_kernel, p);
+    cudaLaunchKernelEx(&config, wide ? attention_join_kernel<true> : attention_join_kernel<false>, p, rows);
     return check_launch("attention_join");
 }
 
