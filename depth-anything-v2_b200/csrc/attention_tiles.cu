@@ -23,7 +23,8 @@
 //                    ring of 128-key tiles; warp 11 rows of Q (TMA where the heads of a
 //                    group divide 128, else copies)
 //   codes:           warp 8 products of both; warps 9-11 int8 from the pages to f16 in
-//                    the same ring, and rows of Q, scaled by a power of two into f16's range
+//                    the same ring; the softmax warps bring Q, scaled by a power of two for
+//                    each row into f16's range
 // The 128-byte-swizzled tiles are 64 dims wide; heads above 64 take two of them.
 //
 // Keys past the end: scores are replaced by -inf; the rows of V behind the last
@@ -68,14 +69,13 @@ constexpr int kEmulated = 2;
 template <int D, bool kS8>
 struct Layout {
     static constexpr uint32_t kOperand = D / 64 * kAtom;   // bytes of 128 rows
-    static constexpr uint32_t kQBufs = D == 64 ? 2 : 1;    // Q of this unit and the next
+    static constexpr uint32_t kQBufs = D == 64 && !kS8 ? 2 : 1;  // Q of this unit and the next
     static constexpr uint32_t kStages = kS8 ? (D == 64 ? 5 : 3) : (D == 64 ? 8 : 5);  // K or V tiles of 16 bits
     static constexpr uint32_t kRaw = kS8 ? 4 : 0;          // tiles of codes in flight
     static constexpr uint32_t kRawBytes = D * kKeys;
-    static constexpr uint32_t kBackSlots = 2 * kQBufs;     // codes: units whose row factors are kept
-    static constexpr uint32_t kBars = 512;                  // bytes of barriers
+    static constexpr uint32_t kBars = 512;                 // bytes of barriers
     static constexpr uint32_t kSmem =
-        (2 * kQBufs + kStages) * kOperand + kRaw * kRawBytes + kBars + (kS8 ? kBackSlots * 2 * kTileRows : 0);
+        (2 * kQBufs + kStages) * kOperand + kRaw * kRawBytes + kBars;
     // Tensor memory columns: S_0, S_1, O_0, O_1, and at D = 64 P_0, P_1; at D = 128,
     // where S and O fill it, P_t takes the first half of S_t.
     static constexpr bool kAlias = D == 128;
@@ -259,19 +259,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* p_full = s_free + 2;       // [tile]
     uint64_t* pv_done = p_full + 2;      // [tile]
     uint64_t* o_full = pv_done + 2;      // [tile]
-    uint64_t* q_full = o_full + 2;       // [buffer]
+    uint64_t* q_full = o_full + 2;       // [buffer]; codes: [tile]
     uint64_t* q_empty = q_full + 2;      // [buffer]
     uint64_t* unit_full = q_empty + 2;   // [response]
     uint64_t* unit_empty = unit_full + 2;  // [response]
     uint64_t* turn = unit_empty + 2;     // [tile]
     uint64_t* drain = turn + 2;
-    uint64_t* raw_full = drain + 2;      // [raw slot]
+    uint64_t* top_full = drain + 2;      // codes: [unit % 4]
+    uint64_t* raw_full = top_full + 4;   // [raw slot]
     uint64_t* raw_empty = raw_full + 4;  // [raw slot]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* s_top = reinterpret_cast<float*>(tmem_slot + 4);        // codes: [slot] the largest V scale
-    int8_t* s_back = reinterpret_cast<int8_t*>(control + L::kBars);  // codes: [slot][row] powers of two of Q
-    static_assert(32 + 8 * (2 * kStages + 30) + 32 <= L::kBars, "barriers overflow their part");
+    float* s_top = reinterpret_cast<float*>(tmem_slot + 4);  // codes: [unit % 4] the largest V scale
+    static_assert(32 + 8 * (2 * kStages + 34) + 32 <= L::kBars, "barriers overflow their part");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if ((smem_addr(smem) & 1023u) != 0) {  // the 128-byte swizzle needs 1 KB aligned tiles
@@ -290,12 +290,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&pv_done[t], 1);
             mbar_init(&o_full[t], 1);
             mbar_init(&turn[t], 1);
-            mbar_init(&q_full[t], kS8 ? kConverters : 1);
+            mbar_init(&q_full[t], kS8 ? 4 : 1);
             mbar_init(&q_empty[t], kIssuers<D, kS8>);
             mbar_init(&unit_full[t], 1);
             mbar_init(&unit_empty[t], kSoftmaxWarps + kIssuers<D, kS8> + (kS8 ? kConverters : 2));  // warps at work
         }
         for (uint32_t i = 0; kS8 && i < 4; ++i) {
+            mbar_init(&top_full[i], 1);
             mbar_init(&raw_full[i], 1);
             mbar_init(&raw_empty[i], kConverters);
         }
@@ -357,18 +358,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t iter = 0;; ++iter) {
             if (iter && !next_unit(iter - 1, u)) break;
             const Unit w = unit_at(p, n, u);
-            if (!w.any) continue;
+            if (!w.any) {
+                if (!iter) break;
+                continue;
+            }
             const uint32_t row = w.row0 + t * kTileRows + r;  // row of the sequence
             const bool live = row < w.where.rows;
             if (!w.blocks) {  // no key in reach
-                if (t >= w.tiles || !live) continue;
-                if (p.splits > 1) {
-                    p.part_ml[part_at(p, w.where, w.kv_head, row, w.split)] = make_float2(-INFINITY, 0.0f);
-                } else {
-                    const uint64_t at = row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
-                    const float zero[2] = {0.0f, 0.0f};
-                    for (uint32_t i = 0; i < p.head_dim; i += 2) store_out(p, at + i, zero, 2);
+                if (t < w.tiles && live) {
+                    if (p.splits > 1) {
+                        p.part_ml[part_at(p, w.where, w.kv_head, row, w.split)] = make_float2(kLowest, 0.0f);
+                    } else {
+                        const uint64_t at = row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
+                        const float zero[2] = {0.0f, 0.0f};
+                        for (uint32_t i = 0; i < p.head_dim; i += 2) store_out(p, at + i, zero, 2);
+                    }
                 }
+                if (!iter) break;
                 continue;
             }
             const uint32_t unit = units++;
@@ -376,9 +382,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             // a negative scale is in the first product's sign; above 0, so that the -inf of a masked key stays
             float c = fmaxf(fabsf(p.scale_log2), 1e-35f), v_top = 1.0f;
             if constexpr (kS8) {
-                if (!warp_wait(&q_full[unit % kQBufs], unit / kQBufs)) break;
-                c *= __uint_as_float((uint32_t)(127 - s_back[unit % L::kBackSlots * 2 * kTileRows + t * kTileRows + r]) << 23);
-                v_top = s_top[unit % L::kBackSlots];
+                // this row of Q, brought into f16's range by a power of two. The last unit's
+                // products are done: this warp has waited for its output.
+                const uint16_t* q = static_cast<const uint16_t*>(p.q) +
+                                    (live ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) : 0);
+                uint4 x[D / 8];
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    x[i] = live && 8 * i < p.head_dim ? *reinterpret_cast<const uint4*>(q + 8 * i) : make_uint4(0, 0, 0, 0);
+                uint32_t* y = reinterpret_cast<uint32_t*>(x);
+                float most = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i) {
+                    const float2 v = unpack2(y[i], p.q_bf16);
+                    most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+                }
+                int ex = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
+                ex = max(-120, min(120, ex));
+                const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
+                c *= __uint_as_float((uint32_t)(127 - ex) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 2; ++i) {
+                    const float2 v = unpack2(y[i], p.q_bf16);
+                    y[i] = pack2<false>(v.x * up, v.y * up);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(sQ + t * L::kOperand + chunk_at(r, i)) = x[i];
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[t]);
+                if (!warp_wait(&top_full[unit & 3u], unit >> 2)) break;
+                v_top = s_top[unit & 3u];
             }
             // where the row's result goes, found now: the unit's numbers need no registers later
             const uint64_t at = !live ? 0
@@ -558,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t role = warp - kSoftmaxWarps;
         uint32_t units = 0, stage = 0, phase = 0;  // stage and phase of the unit's next tile in the ring
         uint32_t done0 = 0, done1 = 0;             // blocks of each tile before this unit
-        uint32_t turns = 0;                        // blocks of units with two tiles
+        uint32_t turns = 0, pairs = 0;             // blocks of units with two tiles; such units
         auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
             return mbar_wait(bar, parity & 1u, abort_flag, p.err);
         };
@@ -600,7 +634,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t iter = 0;; ++iter) {
             if (iter && !next_unit(iter - 1, u)) break;
             const Unit w = unit_at(p, n, u);
-            if (!w.blocks) continue;
+            if (!w.blocks) {
+                if (!iter) break;
+                continue;
+            }
             const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
             const uint32_t tiles = w.tiles, blocks = w.blocks;
             const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
@@ -610,11 +647,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t t0 = kIssuers<D, kS8> == 2 ? role : 0;
                 const uint32_t t1 = kIssuers<D, kS8> == 2 ? min(t0 + 1, tiles) : tiles;
                 const bool take_turns = kTurns<D> && kIssuers<D, kS8> == 2 && tiles == 2;
-                ok = wait(&q_full[qb], units / kQBufs) && wait(&full[stage], phase);
+                ok = (kS8 || wait(&q_full[qb], units / kQBufs)) && wait(&full[stage], phase);
 #pragma unroll 1
                 for (uint32_t t = t0; t < t1 && ok; ++t) {
+                    if (kS8) ok = wait(&q_full[t], t ? pairs : units);
                     const uint32_t before = t ? done1 : done0;
-                    if (!L::kAlias && before) ok = wait(&s_free[t], before - 1);
+                    if (!L::kAlias && before) ok = ok && wait(&s_free[t], before - 1);
                     tc_fence_after();
                     if (ok) issue_s(t, q, stage);
                 }
@@ -678,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             done0 += blocks;
-            if (tiles == 2) done1 += blocks, turns += blocks;
+            if (tiles == 2) done1 += blocks, turns += blocks, ++pairs;
             ++units;
             __syncwarp();
             if (!__shfl_sync(0xffffffffu, ok, 0)) break;
@@ -694,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = true;
                 if (lane == 0) {
                     const int k_batch = p.k_batch ? (int)w.where.seq : 0, v_batch = p.v_batch ? (int)w.where.seq : 0;
-                    if (!w.blocks) ok = ask(iter);
+                    if (!w.blocks) ok = iter && ask(iter);  // a block whose first unit is empty leaves
                     for (uint32_t i = 0; i < 2 * w.blocks; ++i) {
                         const uint32_t at = ring + i, st = at % kStages;
                         if (i == min(kStages + 1, 2 * w.blocks - 1)) ok = ask(iter);
@@ -719,7 +757,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (uint32_t iter = 0;; ++iter) {
                 if (iter && !next_unit(iter - 1, u)) break;
                 const Unit w = unit_at(p, n, u);
-                if (!w.blocks) continue;
+                if (!w.blocks) {
+                    if (!iter) break;
+                    continue;
+                }
                 const uint32_t qb = units % kQBufs;
                 if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
                 ++units;
@@ -771,6 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (iter && !next_unit(iter - 1, u)) break;
             const Unit w = unit_at(p, n, u);
             if (!w.blocks) {
+                if (!iter) break;  // a block whose first unit is empty leaves
                 if (i0 == 0) ok = ask(iter);
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 continue;
@@ -816,65 +858,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             for (uint32_t i = turn_of; ok && i < min(count, L::kRaw); i += kConverters) ok = fetch(i);
             if (!ok) break;
-            // the largest V scale of the keys in reach
-            float v_top = 1e-30f;
-            const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
-            for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
-                const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
-                if (page >= 0 && (uint32_t)page < p.pages)
-                    v_top = fmaxf(v_top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
+            // the largest V scale of the keys in reach. The ring's tiles are those of at most
+            // three units, so that the slot's last value has been read.
+            if (turn_of == 0) {
+                float top = 1e-30f;
+                const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
+#pragma unroll 4
+                for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
+                    const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
+                    if (page >= 0 && (uint32_t)page < p.pages)
+                        top = fmaxf(top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
+                }
+                top = warp_max(top);
+                if (lane == 0) {
+                    s_top[units & 3u] = top;
+                    mbar_arrive(&top_full[units & 3u]);
+                }
+                __syncwarp();
             }
-            v_top = warp_max(v_top);
-            // rows of Q, brought into f16's range by a power of two each: D / 8 lanes to a row,
-            // eight loads of a lane under way
-            const uint32_t qb = units % kQBufs;
-            if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
-            int8_t* back = s_back + units % L::kBackSlots * 2 * kTileRows;
-            if (i0 == 0) s_top[units % L::kBackSlots] = v_top;
-            uint8_t* to_q = sQ + qb * 2 * L::kOperand;
             ++units;
-            constexpr uint32_t kLanes = D / 8, kRows = 32 / kLanes;  // of a row; rows of a load
-            const uint32_t chunk = lane % kLanes;
-#pragma unroll 1
-            for (uint32_t r0 = i0 / 32 * 8 * kRows; r0 < w.tiles * kTileRows; r0 += kConverters * 8 * kRows) {
-                uint4 x[8];
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t r = r0 + k * kRows + lane / kLanes, row = w.row0 + r;
-                    x[k] = make_uint4(0, 0, 0, 0);
-                    if (r < w.tiles * kTileRows && row < w.where.rows && 8 * chunk < p.head_dim)
-                        x[k] = *reinterpret_cast<const uint4*>(
-                            static_cast<const uint16_t*>(p.q) +
-                            row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) + 8 * chunk);
-                }
-#pragma unroll
-                for (uint32_t k = 0; k < 8; ++k) {
-                    const uint32_t r = r0 + k * kRows + lane / kLanes;
-                    uint32_t* y = reinterpret_cast<uint32_t*>(&x[k]);
-                    float most = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = unpack2(y[e], p.q_bf16);
-                        most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
-                    }
-#pragma unroll
-                    for (uint32_t o = kLanes / 2; o; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                    int ex = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
-                    ex = max(-120, min(120, ex));
-                    const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float2 v = unpack2(y[e], p.q_bf16);
-                        y[e] = pack2<false>(v.x * up, v.y * up);
-                    }
-                    if (r >= w.tiles * kTileRows) continue;
-                    if (chunk == 0) back[r] = (int8_t)ex;
-                    *reinterpret_cast<uint4*>(to_q + (r / kTileRows) * L::kOperand + chunk_at(r % kTileRows, chunk)) = x[k];
-                }
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&q_full[qb]);
             for (uint32_t i = 0; ok && i < count; ++i) {
                 const uint32_t at = ring + i, st = at % kStages, slot = at % L::kRaw;
                 ok = warp_wait(&raw_full[slot], at / L::kRaw) && warp_wait(&empty[st], (at / kStages) ^ 1u);
