@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok || !warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
             if (m == kLowest) l = 0.0f;  // a row that sees nothing: its P is 0 or, emulated, 2^-126
+            if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
             const float unit_v = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
             const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
             const float f = l != 0.0f ? (p.splits == 1 ? unit_v / l : unit_v * back) : 0.0f;

@@ -439,6 +439,48 @@ def test_cross_attention_nan_stays_where_it_is(cuda, dav2lib, queries, d):
         assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
 
 
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cross_attention_infinite_scores(cuda, dav2lib, queries, d):
+    """A score of inf makes the row NaN, as inf - inf does in the formula; one of -inf leaves its key out."""
+    g = gen(18)
+    q, k, v = (randn(g, 1, n, 2, d, dtype=torch.bfloat16) for n in (queries, 150, 150))
+    for key in range(0, 150, 7):
+        kk = k.clone()
+        kk[0, key, 1, 5] = math.inf
+        out = torch.empty(1, queries, 2, d, device="cuda")
+        cross(dav2lib, q, kk, v, None, 0.125, out)
+        done(dav2lib)
+        lost = torch.zeros(1, queries, 2, dtype=torch.bool, device="cuda")
+        lost[0, :, 1] = ~(q[0, :, 1, 5] < 0)
+        assert out[lost].isnan().all()
+        want, bound = ref.cross_attention(q, k, v, [150], 0.125, 1, 0)
+        rest = [i for i in range(150) if i != key]
+        without = ref.cross_attention(q[:, :, 1:], k[:, rest, 1:], v[:, rest, 1:], [149], 0.125, 1, 0)
+        want[:, :, 1:], bound[:, :, 1:] = without
+        assert ref.outside(out[~lost], want[~lost], bound[~lost]) <= 1
+
+
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cache_attention_infinite_scores(cuda, dav2lib, queries, d):
+    g = gen(19)
+    q = randn(g, queries, 2, d, dtype=torch.float16)
+    hot = q.clone()
+    hot[0, 1, 5] = math.inf
+    for key in range(0, 150, 7):
+        c = Cache(gen(20), [150], 2, d, 32)
+        c.k[..., 5] = -1
+        c.k[c.table[0][key // 32], 1, key % 32, 5] = 1
+        out = torch.empty(queries, 2, d, device="cuda")
+        attend_cache(dav2lib, c, hot, [150], [0, queries], False, out, 0.125)
+        assert out[0, 1].isnan().all()
+        want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, [150], [0, queries], 0.125, False, 0)
+        keep = torch.ones_like(out, dtype=torch.bool)
+        keep[0, 1] = False
+        assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
+
+
 def test_attention_in_captured_graphs(cuda, dav2lib):
     """Large calls captured into two graphs that share a workspace, replayed in turn on a side stream with new inputs."""
     g = gen(18)
