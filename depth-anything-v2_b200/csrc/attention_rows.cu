@@ -12,10 +12,11 @@
 //   S^T[16 keys x 8 rows] = K[16 x d] Q^T[d x 8],  O^T[d x 8] += V^T[d x 16] P^T[16 x 8]
 // so that one query token with up to eight query heads to a key head wastes
 // nothing of the tile. Bound by memory for such rows: the tensor work is then a
-// few percent, and what counts is bytes in flight. Keys and values go straight
-// from global memory to the registers that the products need: the order of dims
-// in q.k and of keys in p.v is free, so each lane loads 16 (8) consecutive bytes
-// of a row and calls them its fragments. S^T's keys are laid so that transposing
+// few percent, and what counts is bytes in flight: each warp has a ring of keys and
+// values in shared memory that it fills with asynchronous copies of its own, two (16-bit
+// rows: three) steps of 16 or 32 keys deep, and waits for no other warp. The order of
+// dims in q.k and of keys in p.v is free, so each lane reads 16 (8) consecutive bytes of
+// a row from it and calls them its fragments. S^T's keys are laid so that transposing
 // P's 8x8 blocks across lanes (movmatrix) gives the second product's operand.
 //
 // Codes become f16 exactly (byte + 1024 by a byte permutation, minus 1152), and q
@@ -29,10 +30,19 @@
 // the unrounded values. 16-bit values take p in their own type, as the tensor
 // core wants both operands alike.
 //
-// A block's four warps take either the same rows and every fourth step of keys, merged
-// at the end in shared memory, or (many rows) four row tiles and the same keys, which
-// they then find in L1. Where there are few row tiles, the keys of a tile are split
-// over several blocks whose (o, m, sum) go to the workspace, and a second kernel joins them.
+// A block's four warps take the same rows and every fourth step of keys, or (more than 16
+// rows) two row tiles and every second step, merged at the end in shared memory. Where
+// there are few row tiles, the keys of a tile are split over several blocks: up to eight
+// are a cluster that joins their (o, m, sum) over its shared memory; more go to the
+// workspace, and a second kernel, launched before the first has ended, joins them.
+//
+// Codes: the conversion shares the issue slots with the loads (of an SM's four
+// instructions a cycle 2.6 are issued, over half of them for integer work), so that the
+// memory is not quite full: 200003 keys, 32 heads of 128 on 8 key heads, in 72 us (5.7
+// TB/s; without the rings 94 us); 48 streams of 2000 to 8192 keys, one token each, 111 us
+// (4.6 TB/s: lengths and waves are uneven). 16-bit rows: 16 streams of up to 1370 keys, 16
+// heads of 64, 15 us (4.6 TB/s). 1370 keys of one stream, 7.8 us: launch, a chain of four
+// dependent loads, and the join.
 #include <algorithm>
 
 #include "attention_rows.cuh"
@@ -66,7 +76,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     return y;
 }
 
-__device__ __forceinline__ uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+__device__ __forceinline__ uint32_t word(const uint4& x, int i) {
+    return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w;
+}
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -19,18 +19,27 @@
 // still write the last unit's rows.
 //
 //   warps 0-3, 4-7   softmax of tile 0, 1
-//   16-bit rows:     warps 8, 9 products (D = 64: S, P V; D = 128: of tile 0, 1); warp 10 TMA of K_j, V_j into a
+//   16-bit rows:     warps 8, 9 products of tile 0, 1; warp 10 TMA of K_j, V_j into a
 //                    ring of 128-key tiles; warp 11 rows of Q (TMA where the heads of a
 //                    group divide 128, else copies)
-//   codes:           warp 8 products of both; warps 9-11 int8 from the pages to f16 in
-//                    the same ring; the softmax warps bring Q, scaled by a power of two for
-//                    each row into f16's range
+//   codes:           warp 8 products of both; warps 9-11 int8 from the pages, by bulk
+//                    copies, to f16 in the same ring; the softmax warps bring Q, scaled by
+//                    a power of two for each row into f16's range
 // The 128-byte-swizzled tiles are 64 dims wide; heads above 64 take two of them.
 //
 // Keys past the end: scores are replaced by -inf; the rows of V behind the last
 // key are set to zero in shared memory before the last product, as they may hold
 // NaN. Codes: K's scale multiplies the scores of its page's keys, V's scale, over
 // the largest of the sequence, multiplies P before it is rounded.
+//
+// Bound by the softmax: for 128 keys an SM's four exponential units need 1.1 us at D = 64 and
+// 128 alike (0.8 with the polynomials), the products 0.65 and 1.1 us, and each tile's chain from
+// its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
+// other's alone.
+// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 138 us (446 TFLOP/s); 4 x 1370 x 5477, 16
+// heads of 128 on 4 key heads, padded batch, 216 us (890 TFLOP/s). Codes: the chain of one
+// issuer and the conversion on top; 700 queries over 6 caches of up to 6000 tokens, 32 heads
+// of 128 on 8 key heads, 134 us (298 TFLOP/s).
 // Every wait is bounded (kWaitTimeoutNs); a timeout sets the device error word.
 #include <cudaTypedefs.h>
 
@@ -48,23 +57,37 @@ constexpr uint32_t kKeys = 128;        // keys of a block
 constexpr uint32_t kAtom = 128 * 128;  // bytes of 128 rows x 64 dims of 16 bits
 constexpr float kRaise = 8.0f;
 constexpr uint32_t kSoftmaxWarps = 8;
-constexpr uint32_t kConverters = 3;      // codes
-constexpr uint32_t kThreads = 12 * 32;   // 168 registers each
+constexpr uint32_t kConverters = 3;     // codes
+constexpr uint32_t kThreads = 12 * 32;  // 168 registers each at launch
+// What the softmax warps, whose rows of 128 scores want more than that, take over from the
+// other four: 8 x 32 x (208 - 168) = 4 x 32 x (168 - 88), codes 8 x 32 x (200 - 168) = 4 x
+// 32 x (168 - 104), as the converters keep a batch of codes in registers. With 168 for all, 100
+// to 290 bytes of spills: 8 x 1370 x 1370, 16 heads of 64, 143 us for 138; 700 queries over
+// caches of up to 6000 tokens, 32 heads of 128, 149 us for 143.
+template <bool kS8>
+constexpr uint32_t kSoftmaxRegisters = kS8 ? 200 : 208;
+template <bool kS8>
+constexpr uint32_t kOtherRegisters = kS8 ? 104 : 88;
+static_assert(2 * kSoftmaxRegisters<false> + kOtherRegisters<false> <= 3 * 168 &&
+                  2 * kSoftmaxRegisters<true> + kOtherRegisters<true> <= 3 * 168,
+              "more registers than the block is launched with");
 // Warps that issue products: one for each tile, so that what one does between its
 // products is hidden by the other's. Codes need the second warp for conversion.
 template <int D, bool kS8>
 constexpr uint32_t kIssuers = kS8 ? 1 : 2;
 // At D = 128, where S waits for P, the two take turns: products that interleave bring the
 // tiles into step, so that both softmaxes and then both products wait (128 x 5477 keys:
-// 98 us, without turns 130 us). At D = 64, where S runs ahead, turns cost 7%.
+// 97 us, without turns 130 us). At D = 64, where S runs ahead, turns gain nothing.
 template <int D>
 constexpr bool kTurns = D == 128;
 
 constexpr float kLowest = -3.402823466e38f;
 // Of eight pairs of exponentials, how many leave the exponential unit alone. Measured with
-// 0, 1, 2, 3, 4 of 8: 8 x 1370 x 1370, 16 heads of 64, 148, 141, 138, 142, 152 us; 4 x 1370 x
-// 5477, 16 heads of 128, 233, 229, 237, 231, 268 us.
-constexpr int kEmulated = 2;
+// 0, 1, 2, 3 of 8: 8 x 1370 x 1370, 16 heads of 64, 157, 142, 143, 140 us; 4 x 1370 x 5477,
+// 16 heads of 128, 229, 222, 221, 244 us. Codes, whose softmax shares the issue slots with the
+// conversion, are slower with any: 149, 151, 153, 156 us (700 queries over 6 caches).
+template <bool kS8>
+constexpr int kEmulated = kS8 ? 0 : 2;
 
 template <int D, bool kS8>
 struct Layout {
@@ -143,7 +166,8 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // 2^x of two values without the exponential unit, which the softmax would otherwise be
 // bound by (a quarter of the rate of a multiply-add): x = n + f with |f| <= 1/2, a
 // polynomial of degree 4 for 2^f (minimax in the relative error, 2.7e-6 as evaluated),
-// and n added to the exponent. x <= 127; below -126 the result is 2^-126.
+// and n added to the exponent. x <= 127; below -126 the result is 2^-126, not 0, which a bf16 P
+// keeps: beside other values of V it counts where a value is above 2^100 times theirs.
 __device__ __forceinline__ void exp2_pair(float& x, float& y) {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it leaves rint(x) in the low bits
     x = fmaxf(x, -126.0f), y = fmaxf(y, -126.0f);
@@ -345,6 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp < kSoftmaxWarps) {
         // ------------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegisters<kS8>));
         const uint32_t t = warp >> 2, quarter = warp & 3u;
         const uint32_t r = quarter * 32u + lane;  // row of the tile
         const uint32_t lanes = (quarter * 32u) << 16;
@@ -461,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int i = 0; i < 8; ++i) {
                         const float f = __shfl_sync(0xffffffffu, scale_now, i) * c;
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) f2_mul(s[16 * i + e], s[16 * i + e + 1], s[16 * i + e], s[16 * i + e + 1], f, f);
+                        for (int e = 16 * i; e < 16 * i + 16; e += 2) f2_mul(s[e], s[e + 1], s[e], s[e + 1], f, f);
                     }
                     if (__any_sync(0xffffffffu, scale_now < 0.0f)) {  // keys of no page of the cache
 #pragma unroll
@@ -528,7 +553,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float x = s[64 * h + 2 * i], y = s[64 * h + 2 * i + 1];
                         if constexpr (kS8) f2_add(x, y, x, y, off, off);
                         else f2_fma(x, y, x, y, c, c, off, off);
-                        if (i % 8 < kEmulated) exp2_pair(x, y);
+                        if (i % 8 < kEmulated<kS8>) exp2_pair(x, y);
                         else x = ex2_approx(x), y = ex2_approx(y);
                         f2_add(ls[(2 * i) & 3], ls[(2 * i + 1) & 3], ls[(2 * i) & 3], ls[(2 * i + 1) & 3], x, y);
                         if constexpr (kS8) f2_mul(x, y, x, y, sv[i / 8], sv[i / 8]);
@@ -581,179 +606,58 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tc_fence_before();  // O is read: the next unit's first product, after its P, may overwrite it
         }
-    } else if (warp < kSoftmaxWarps + kIssuers<D, kS8>) {
-        // ----------------------------------------------------------- products
-        // One thread issues, with everything but the waits unrolled: between its products the
-        // tensor cores may wait, as their queue holds a few (rolled up, 5 to 15% slower).
-        constexpr uint32_t ab = kBF16 ? 1u : 0u;
-        const uint32_t idesc_s = make_idesc(1u, ab, 128u, 128u) | (p.scale_log2 < 0.0f ? 1u << 13 : 0u);  // or -Q
-        constexpr uint32_t idesc_o = make_idesc(1u, ab, 128u, D) | (1u << 16);  // V is MN-major
-        constexpr uint32_t kStageDesc = L::kOperand >> 4;
-        const uint32_t kv_base = smem_addr(sKV) >> 4, q_all = (smem_addr(sQ) >> 4) | kDescK;
-        const uint32_t role = warp - kSoftmaxWarps;
-        uint32_t units = 0, stage = 0, phase = 0;  // stage and phase of the unit's next tile in the ring
-        uint32_t done0 = 0, done1 = 0;             // blocks of each tile before this unit
-        uint32_t turns = 0, pairs = 0;             // blocks of units with two tiles; such units
-        auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-            return mbar_wait(bar, parity & 1u, abort_flag, p.err);
-        };
-        auto next_stage = [&](uint32_t by) {
-            stage += by;
-            if (stage >= kStages) stage -= kStages, phase ^= 1u;
-        };
-        auto issue_s = [&](uint32_t t, uint32_t q, uint32_t st) {
-            q += t * kStageDesc;
-            const uint32_t k = kv_base + st * kStageDesc + kDescK, d = tmem + 128u * t;
-            umma_ss<false>(d, q, k, idesc_s);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegisters<kS8>));
+        if (warp < kSoftmaxWarps + kIssuers<D, kS8>) {
+            // ----------------------------------------------------------- products
+            // One thread issues, with everything but the waits unrolled: between its products the
+            // tensor cores may wait, as their queue holds a few (rolled up, 5 to 15% slower).
+            constexpr uint32_t ab = kBF16 ? 1u : 0u;
+            const uint32_t idesc_s = make_idesc(1u, ab, 128u, 128u) | (p.scale_log2 < 0.0f ? 1u << 13 : 0u);  // or -Q
+            constexpr uint32_t idesc_o = make_idesc(1u, ab, 128u, D) | (1u << 16);  // V is MN-major
+            constexpr uint32_t kStageDesc = L::kOperand >> 4;
+            const uint32_t kv_base = smem_addr(sKV) >> 4, q_all = (smem_addr(sQ) >> 4) | kDescK;
+            const uint32_t role = warp - kSoftmaxWarps;
+            uint32_t units = 0, stage = 0, phase = 0;  // stage and phase of the unit's next tile in the ring
+            uint32_t done0 = 0, done1 = 0;             // blocks of each tile before this unit
+            uint32_t turns = 0, pairs = 0;             // blocks of units with two tiles; such units
+            auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+                return mbar_wait(bar, parity & 1u, abort_flag, p.err);
+            };
+            auto next_stage = [&](uint32_t by) {
+                stage += by;
+                if (stage >= kStages) stage -= kStages, phase ^= 1u;
+            };
+            auto issue_s = [&](uint32_t t, uint32_t q, uint32_t st) {
+                q += t * kStageDesc;
+                const uint32_t k = kv_base + st * kStageDesc + kDescK, d = tmem + 128u * t;
+                umma_ss<false>(d, q, k, idesc_s);
 #pragma unroll
-            for (uint32_t kk = 1; kk < D / 16; ++kk) {
-                const uint32_t off = ((kk / 4) * kAtom + 32u * (kk % 4)) >> 4;
-                umma_ss<true>(d, q + off, k + off, idesc_s);
-            }
-            umma_commit(&s_full[t]);
-        };
-        auto issue_o = [&](uint32_t t, uint32_t st, uint32_t steps, uint32_t later) {
-            const uint32_t o = tmem + L::kO + t * D, pt = tmem + L::kP + t * L::kPStride;
-            const uint32_t v = kv_base + st * kStageDesc + kDescV;
-            if (steps == 8) {
-                umma_ts(o, pt, v, idesc_o, later);
+                for (uint32_t kk = 1; kk < D / 16; ++kk) {
+                    const uint32_t off = ((kk / 4) * kAtom + 32u * (kk % 4)) >> 4;
+                    umma_ss<true>(d, q + off, k + off, idesc_s);
+                }
+                umma_commit(&s_full[t]);
+            };
+            auto issue_o = [&](uint32_t t, uint32_t st, uint32_t steps, uint32_t later) {
+                const uint32_t o = tmem + L::kO + t * D, pt = tmem + L::kP + t * L::kPStride;
+                const uint32_t v = kv_base + st * kStageDesc + kDescV;
+                if (steps == 8) {
+                    umma_ts(o, pt, v, idesc_o, later);
 #pragma unroll
-                for (uint32_t kk = 1; kk < 8; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, 1u);
-            } else {
-                for (uint32_t kk = 0; kk < steps; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, later | kk);
-            }
-        };
-        // rows of V behind the last key, up to the product's end
-        auto clear_tail = [&](uint32_t st, uint32_t valid) {
-            uint8_t* v = sKV + st * L::kOperand;
-#pragma unroll 1
-            for (uint32_t i = 0; i < (16u - (valid & 15u)) * (D / 8); ++i)
-                *reinterpret_cast<uint4*>(v + chunk_at(valid + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
-            fence_async_smem();
-        };
-        uint32_t u = blockIdx.x;
-        for (uint32_t iter = 0;; ++iter) {
-            if (iter && !next_unit(iter - 1, u)) break;
-            const Unit w = unit_at(p, n, u);
-            if (!w.blocks) {
-                if (!iter) break;
-                continue;
-            }
-            const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
-            const uint32_t tiles = w.tiles, blocks = w.blocks;
-            const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
-            bool ok = true;
-            if (lane == 0) {
-                mma_issued = true;
-                const uint32_t t0 = kIssuers<D, kS8> == 2 ? role : 0;
-                const uint32_t t1 = kIssuers<D, kS8> == 2 ? min(t0 + 1, tiles) : tiles;
-                const bool take_turns = kTurns<D> && kIssuers<D, kS8> == 2 && tiles == 2;
-                ok = (kS8 || wait(&q_full[qb], units / kQBufs)) && wait(&full[stage], phase);
-#pragma unroll 1
-                for (uint32_t t = t0; t < t1 && ok; ++t) {
-                    if (kS8) ok = wait(&q_full[t], t ? pairs : units);
-                    const uint32_t before = t ? done1 : done0;
-                    if (!L::kAlias && before) ok = ok && wait(&s_free[t], before - 1);
-                    tc_fence_after();
-                    if (ok) issue_s(t, q, stage);
+                    for (uint32_t kk = 1; kk < 8; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, 1u);
+                } else {
+                    for (uint32_t kk = 0; kk < steps; ++kk) umma_ts(o, pt + 8u * kk, v + 128u * kk, idesc_o, later | kk);
                 }
-                if (t0 < t1) {
-                    umma_commit(&empty[stage]);
-                    if (blocks == 1) umma_commit(&q_empty[qb]);
-                } else if (ok) {  // no rows of this tile: its stages are released as they are filled
-                    mbar_arrive(&empty[stage]);
-                    mbar_arrive(&q_empty[qb]);
-                }
-                next_stage(1);
+            };
+            // rows of V behind the last key, up to the product's end
+            auto clear_tail = [&](uint32_t st, uint32_t valid) {
+                uint8_t* v = sKV + st * L::kOperand;
 #pragma unroll 1
-                for (uint32_t j = 0; ok && j < blocks; ++j) {
-                    const bool more = j + 1 < blocks;
-                    const uint32_t sv = stage;
-                    ok = wait(&full[sv], phase);
-                    next_stage(1);
-                    const uint32_t sk = stage;
-                    if (more) {
-                        ok = ok && wait(&full[sk], phase);
-                        next_stage(1);
-                    }
-                    if (t0 >= t1) {
-                        if (!ok) break;
-                        mbar_arrive(&empty[sv]);
-                        if (more) mbar_arrive(&empty[sk]);
-                        continue;
-                    }
-                    const uint32_t valid = more ? kKeys : last_keys;
-                    if (ok && !kS8 && (valid & 15u)) clear_tail(sv, valid);
-                    // S of the next block: beside this block's softmax where P has its own columns
-                    if (!L::kAlias && more) {
-#pragma unroll 1
-                        for (uint32_t t = t0; t < t1 && ok; ++t) {
-                            ok = wait(&s_free[t], (t ? done1 : done0) + j);
-                            tc_fence_after();
-                            if (ok) issue_s(t, q, sk);
-                        }
-                        umma_commit(&empty[sk]);
-                        if (j + 2 == blocks) umma_commit(&q_empty[qb]);
-                    }
-#pragma unroll 1
-                    for (uint32_t t = t0; t < t1 && ok; ++t) {
-                        ok = wait(&p_full[t], (t ? done1 : done0) + j);
-                        // the tiles' products one after the other, not interleaved: tile 0 of
-                        // block j, tile 1 of block j, tile 0 of block j + 1
-                        if (take_turns && ok && (t || turns + j)) ok = wait(&turn[t], t ? turns + j : turns + j - 1);
-                        tc_fence_after();
-                        if (!ok) break;
-                        issue_o(t, sv, (valid + 15u) / 16u, j);
-                        if (L::kAlias && more) issue_s(t, q, sk);
-                        if (take_turns) mbar_arrive(&turn[t ^ 1u]);
-                        if (!L::kAlias) umma_commit(&pv_done[t]);
-                        if (!more) umma_commit(&o_full[t]);
-                    }
-                    umma_commit(&empty[sv]);
-                    if (L::kAlias && more) {
-                        umma_commit(&empty[sk]);
-                        if (j + 2 == blocks) umma_commit(&q_empty[qb]);
-                    }
-                }
-            }
-            done0 += blocks;
-            if (tiles == 2) done1 += blocks, turns += blocks, ++pairs;
-            ++units;
-            __syncwarp();
-            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        }
-    } else if constexpr (!kS8) {
-        uint32_t ring = 0, units = 0;
-        if (warp == 10) {
-            // -------------------------------------------------- TMA, and the next unit
-            uint32_t u = blockIdx.x;
-            for (uint32_t iter = 0;; ++iter) {
-                if (iter && !next_unit(iter - 1, u)) break;
-                const Unit w = unit_at(p, n, u);
-                bool ok = true;
-                if (lane == 0) {
-                    const int k_batch = p.k_batch ? (int)w.where.seq : 0, v_batch = p.v_batch ? (int)w.where.seq : 0;
-                    if (!w.blocks) ok = iter && ask(iter);  // a block whose first unit is empty leaves
-                    for (uint32_t i = 0; i < 2 * w.blocks; ++i) {
-                        const uint32_t at = ring + i, st = at % kStages;
-                        if (i == min(kStages + 1, 2 * w.blocks - 1)) ok = ask(iter);
-                        if (!ok || *abort_flag || !mbar_wait(&empty[st], ((at / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
-                            ok = false;
-                            break;
-                        }
-                        mbar_arrive_expect_tx(&full[st], L::kOperand);
-                        const int key0 = (int)((w.first + i / 2) * kKeys);
-#pragma unroll
-                        for (int h = 0; h < D / 64; ++h)
-                            tma_load_4d(sKV + st * L::kOperand + h * kAtom, i & 1 ? &tm_v : &tm_k, &full[st], 64 * h,
-                                        (int)w.kv_head, key0, i & 1 ? v_batch : k_batch);
-                    }
-                }
-                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-                ring += 2 * w.blocks;
-            }
-        } else if (warp == 11) {
-            // -------------------------------------------------------------- Q
+                for (uint32_t i = 0; i < (16u - (valid & 15u)) * (D / 8); ++i)
+                    *reinterpret_cast<uint4*>(v + chunk_at(valid + i / (D / 8), i % (D / 8))) = make_uint4(0, 0, 0, 0);
+                fence_async_smem();
+            };
             uint32_t u = blockIdx.x;
             for (uint32_t iter = 0;; ++iter) {
                 if (iter && !next_unit(iter - 1, u)) break;
@@ -762,159 +666,296 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!iter) break;
                     continue;
                 }
-                const uint32_t qb = units % kQBufs;
-                if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
+                const uint32_t qb = units % kQBufs, q = q_all + qb * 2 * kStageDesc;
+                const uint32_t tiles = w.tiles, blocks = w.blocks;
+                const uint32_t last_keys = min(kKeys, w.len - (w.first + blocks - 1) * kKeys);  // of the last block
+                bool ok = true;
+                if (lane == 0) {
+                    mma_issued = true;
+                    const uint32_t t0 = kIssuers<D, kS8> == 2 ? role : 0;
+                    const uint32_t t1 = kIssuers<D, kS8> == 2 ? min(t0 + 1, tiles) : tiles;
+                    const bool take_turns = kTurns<D> && kIssuers<D, kS8> == 2 && tiles == 2;
+                    ok = (kS8 || wait(&q_full[qb], units / kQBufs)) && wait(&full[stage], phase);
+#pragma unroll 1
+                    for (uint32_t t = t0; t < t1 && ok; ++t) {
+                        if (kS8) ok = wait(&q_full[t], t ? pairs : units);
+                        const uint32_t before = t ? done1 : done0;
+                        if (!L::kAlias && before) ok = ok && wait(&s_free[t], before - 1);
+                        tc_fence_after();
+                        if (ok) issue_s(t, q, stage);
+                    }
+                    if (t0 < t1) {
+                        umma_commit(&empty[stage]);
+                        if (blocks == 1) umma_commit(&q_empty[qb]);
+                    } else if (ok) {  // no rows of this tile: its stages are released as they are filled
+                        mbar_arrive(&empty[stage]);
+                        mbar_arrive(&q_empty[qb]);
+                    }
+                    next_stage(1);
+#pragma unroll 1
+                    for (uint32_t j = 0; ok && j < blocks; ++j) {
+                        const bool more = j + 1 < blocks;
+                        const uint32_t sv = stage;
+                        ok = wait(&full[sv], phase);
+                        next_stage(1);
+                        const uint32_t sk = stage;
+                        if (more) {
+                            ok = ok && wait(&full[sk], phase);
+                            next_stage(1);
+                        }
+                        if (t0 >= t1) {
+                            if (!ok) break;
+                            mbar_arrive(&empty[sv]);
+                            if (more) mbar_arrive(&empty[sk]);
+                            continue;
+                        }
+                        const uint32_t valid = more ? kKeys : last_keys;
+                        if (ok && !kS8 && (valid & 15u)) clear_tail(sv, valid);
+                        // S of the next block: beside this block's softmax where P has its own columns
+                        if (!L::kAlias && more) {
+#pragma unroll 1
+                            for (uint32_t t = t0; t < t1 && ok; ++t) {
+                                ok = wait(&s_free[t], (t ? done1 : done0) + j);
+                                tc_fence_after();
+                                if (ok) issue_s(t, q, sk);
+                            }
+                            umma_commit(&empty[sk]);
+                            if (j + 2 == blocks) umma_commit(&q_empty[qb]);
+                        }
+#pragma unroll 1
+                        for (uint32_t t = t0; t < t1 && ok; ++t) {
+                            ok = wait(&p_full[t], (t ? done1 : done0) + j);
+                            // the tiles' products one after the other, not interleaved: tile 0 of
+                            // block j, tile 1 of block j, tile 0 of block j + 1
+                            if (take_turns && ok && (t || turns + j)) ok = wait(&turn[t], t ? turns + j : turns + j - 1);
+                            tc_fence_after();
+                            if (!ok) break;
+                            issue_o(t, sv, (valid + 15u) / 16u, j);
+                            if (L::kAlias && more) issue_s(t, q, sk);
+                            if (take_turns) mbar_arrive(&turn[t ^ 1u]);
+                            if (!L::kAlias) umma_commit(&pv_done[t]);
+                            if (!more) umma_commit(&o_full[t]);
+                        }
+                        umma_commit(&empty[sv]);
+                        if (L::kAlias && more) {
+                            umma_commit(&empty[sk]);
+                            if (j + 2 == blocks) umma_commit(&q_empty[qb]);
+                        }
+                    }
+                }
+                done0 += blocks;
+                if (tiles == 2) done1 += blocks, turns += blocks, ++pairs;
                 ++units;
-                uint8_t* to = sQ + qb * 2 * L::kOperand;
-                if (n.q_box) {
-                    // 128 rows are q_box tokens of the group's heads
+                __syncwarp();
+                if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+            }
+        } else if constexpr (!kS8) {
+            uint32_t ring = 0, units = 0;
+            if (warp == 10) {
+                // -------------------------------------------------- TMA, and the next unit
+                uint32_t u = blockIdx.x;
+                for (uint32_t iter = 0;; ++iter) {
+                    if (iter && !next_unit(iter - 1, u)) break;
+                    const Unit w = unit_at(p, n, u);
+                    bool ok = true;
                     if (lane == 0) {
-                        mbar_arrive_expect_tx(&q_full[qb], w.tiles * L::kOperand);
-                        const int batch = p.q_batch ? (int)w.where.seq : 0;
-                        for (uint32_t t = 0; t < w.tiles; ++t)
+                        const int k_batch = p.k_batch ? (int)w.where.seq : 0, v_batch = p.v_batch ? (int)w.where.seq : 0;
+                        if (!w.blocks) ok = iter && ask(iter);  // a block whose first unit is empty leaves
+                        for (uint32_t i = 0; i < 2 * w.blocks; ++i) {
+                            const uint32_t at = ring + i, st = at % kStages;
+                            if (i == min(kStages + 1, 2 * w.blocks - 1)) ok = ask(iter);
+                            if (!ok || *abort_flag || !mbar_wait(&empty[st], ((at / kStages) & 1u) ^ 1u, abort_flag, p.err)) {
+                                ok = false;
+                                break;
+                            }
+                            mbar_arrive_expect_tx(&full[st], L::kOperand);
+                            const int key0 = (int)((w.first + i / 2) * kKeys);
 #pragma unroll
                             for (int h = 0; h < D / 64; ++h)
-                                tma_load_4d(to + t * L::kOperand + h * kAtom, &tm_q, &q_full[qb], 64 * h,
-                                            (int)(w.kv_head * p.group), (int)((w.where.tile * 2 + t) * n.q_box), batch);
+                                tma_load_4d(sKV + st * L::kOperand + h * kAtom, i & 1 ? &tm_v : &tm_k, &full[st], 64 * h,
+                                            (int)w.kv_head, key0, i & 1 ? v_batch : k_batch);
+                        }
                     }
-                    __syncwarp();
-                    continue;
+                    if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+                    ring += 2 * w.blocks;
                 }
-                const uint32_t rows = w.tiles * kTileRows;
-#pragma unroll 1
-                for (uint32_t i = lane; i < rows * (D / 8); i += 32) {
-                    const uint32_t r = i / (D / 8), chunk = i % (D / 8), row = w.row0 + r;
-                    const bool read = row < w.where.rows && 8 * chunk < p.head_dim;
-                    const uint16_t* from = static_cast<const uint16_t*>(p.q) +
-                                           (read ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) + 8 * chunk : 0);
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                     smem_addr(to + (r / kTileRows) * L::kOperand + chunk_at(r % kTileRows, chunk))),
-                                 "l"(from), "r"(read ? 16u : 0u)
-                                 : "memory");
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full[qb]);
-            }
-        }
-    } else {
-        // -------------------------------------------------------------- codes
-        // kRaw tiles of codes are under way from the pages (a page's tokens of a head are one
-        // run of bytes, copied in one piece; the three warps start the copies in turn); the
-        // warps turn each into a 16-bit tile, 16 dims of a key at a time.
-        constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
-        const uint32_t i0 = threadIdx.x - 9 * 32;
-        const uint32_t in_page = (1u << p.page_shift) - 1;
-        uint32_t ring = 0, units = 0;
-        bool ok = true;
-        uint32_t u = blockIdx.x;
-        for (uint32_t iter = 0; ok; ++iter) {
-            if (iter && !next_unit(iter - 1, u)) break;
-            const Unit w = unit_at(p, n, u);
-            if (!w.blocks) {
-                if (!iter) break;  // a block whose first unit is empty leaves
-                if (i0 == 0) ok = ask(iter);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                continue;
-            }
-            // lanes 0 to 7 have the page of their piece of a block
-            const uint32_t piece = min(1u << p.page_shift, kKeys);
-            auto page_of = [&](uint32_t j) -> int32_t {
-                const uint32_t in_block = lane * piece, key = (w.first + j) * kKeys + in_block;
-                if (in_block >= kKeys || key >= w.len) return -1;
-                const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
-                if (page < 0 || (uint32_t)page >= p.pages) {
-                    atomicExch(p.err, 3);
-                    return -1;
-                }
-                return page;
-            };
-            const uint32_t count = 2 * w.blocks, turn_of = i0 / 32;
-            int32_t page_next = turn_of < count ? page_of(turn_of / 2) : -1;  // for the warp's next tile
-            // Starts the copies of tile i (K_j: 2j, V_j: 2j + 1). Keys of no page, and past the
-            // end, keep what the slot holds: any byte is a finite code, and they weigh nothing.
-            auto fetch = [&](uint32_t i) -> bool {
-                const uint32_t at = ring + i, slot = at % L::kRaw;
-                if (!warp_wait(&raw_empty[slot], (at / L::kRaw) ^ 1u)) return false;
-                const int32_t page_now = page_next;
-                if (i + kConverters < count) page_next = page_of((i + kConverters) / 2);
-                const uint32_t bytes = piece * p.head_dim;
-                const uint32_t live = __popc(__ballot_sync(0xffffffffu, page_now >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], live * bytes);
-                __syncwarp();
-                if (page_now >= 0) {
-                    const uint32_t key = (w.first + i / 2) * kKeys + lane * piece;
-                    const int8_t* from =
-                        static_cast<const int8_t*>(i & 1 ? p.v : p.k) +
-                        ((((uint64_t)page_now * p.kv_heads + w.kv_head) << p.page_shift) + (key & in_page)) * p.head_dim;
-                    asm volatile(
-                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                            smem_addr(sRaw + slot * L::kRawBytes + lane * bytes)),
-                        "l"(from), "r"(bytes), "r"(smem_addr(&raw_full[slot]))
-                        : "memory");
-                }
-                __syncwarp();
-                return true;
-            };
-            for (uint32_t i = turn_of; ok && i < min(count, L::kRaw); i += kConverters) ok = fetch(i);
-            if (!ok) break;
-            // the largest V scale of the keys in reach. The ring's tiles are those of at most
-            // three units, so that the slot's last value has been read.
-            if (turn_of == 0) {
-                float top = 1e-30f;
-                const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
-#pragma unroll 4
-                for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
-                    const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
-                    if (page >= 0 && (uint32_t)page < p.pages)
-                        top = fmaxf(top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
-                }
-                top = warp_max(top);
-                if (lane == 0) {
-                    s_top[units & 3u] = top;
-                    mbar_arrive(&top_full[units & 3u]);
-                }
-                __syncwarp();
-            }
-            ++units;
-            for (uint32_t i = 0; ok && i < count; ++i) {
-                const uint32_t at = ring + i, st = at % kStages, slot = at % L::kRaw;
-                ok = warp_wait(&raw_full[slot], at / L::kRaw) && warp_wait(&empty[st], (at / kStages) ^ 1u);
-                if (!ok) break;
-                uint8_t* to = sKV + st * L::kOperand;
-                const uint8_t* from = sRaw + slot * L::kRawBytes;
+            } else if (warp == 11) {
+                // -------------------------------------------------------------- Q
+                uint32_t u = blockIdx.x;
+                for (uint32_t iter = 0;; ++iter) {
+                    if (iter && !next_unit(iter - 1, u)) break;
+                    const Unit w = unit_at(p, n, u);
+                    if (!w.blocks) {
+                        if (!iter) break;
+                        continue;
+                    }
+                    const uint32_t qb = units % kQBufs;
+                    if (!warp_wait(&q_empty[qb], (units / kQBufs) ^ 1u)) break;
+                    ++units;
+                    uint8_t* to = sQ + qb * 2 * L::kOperand;
+                    if (n.q_box) {
+                        // 128 rows are q_box tokens of the group's heads
+                        if (lane == 0) {
+                            mbar_arrive_expect_tx(&q_full[qb], w.tiles * L::kOperand);
+                            const int batch = p.q_batch ? (int)w.where.seq : 0;
+                            for (uint32_t t = 0; t < w.tiles; ++t)
 #pragma unroll
-                for (uint32_t k = 0; k < (kKeys * kParts + kStep - 1) / kStep; ++k) {
-                    // eight lanes: four dims' parts of two rows, at D = 128 the first half of one and
-                    // the second of the other, which spreads loads and stores over the banks
-                    const uint32_t at16 = i0 + kStep * k;
-                    const uint32_t key = D == 64 ? at16 / 4 : at16 / 16 * 2 + (at16 / 4 & 1);
-                    const uint32_t part = D == 64 ? at16 % 4 : at16 % 4 + 4 * ((at16 / 4 ^ at16 / 8) & 1);
-                    if (key >= kKeys) continue;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (16 * part < p.head_dim) x = *reinterpret_cast<const uint4*>(from + key * p.head_dim + 16 * part);
-                    const uint32_t w4[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
-                    *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part)) =
-                        make_uint4(codes_lo(w4[0]), codes_hi(w4[0]), codes_lo(w4[1]), codes_hi(w4[1]));
-                    *reinterpret_cast<uint4*>(to + chunk_at(key, 2 * part + 1)) =
-                        make_uint4(codes_lo(w4[2]), codes_hi(w4[2]), codes_lo(w4[3]), codes_hi(w4[3]));
+                                for (int h = 0; h < D / 64; ++h)
+                                    tma_load_4d(to + t * L::kOperand + h * kAtom, &tm_q, &q_full[qb], 64 * h,
+                                                (int)(w.kv_head * p.group), (int)((w.where.tile * 2 + t) * n.q_box), batch);
+                        }
+                        __syncwarp();
+                        continue;
+                    }
+                    const uint32_t rows = w.tiles * kTileRows;
+#pragma unroll 1
+                    for (uint32_t i = lane; i < rows * (D / 8); i += 32) {
+                        const uint32_t r = i / (D / 8), chunk = i % (D / 8), row = w.row0 + r;
+                        const bool read = row < w.where.rows && 8 * chunk < p.head_dim;
+                        const uint16_t* from = static_cast<const uint16_t*>(p.q) +
+                                               (read ? row_at(p, w.where, w.kv_head, row, p.q_batch, p.q_stride) + 8 * chunk : 0);
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_addr(to + (r / kTileRows) * L::kOperand + chunk_at(r % kTileRows, chunk))),
+                                     "l"(from), "r"(read ? 16u : 0u)
+                                     : "memory");
+                    }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_full[qb]);
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&full[st]);
-                    mbar_arrive(&raw_empty[slot]);
-                }
-                if (i == min(4u, count - 1)) {
+            }
+        } else {
+            // -------------------------------------------------------------- codes
+            // kRaw tiles of codes are under way from the pages (a page's tokens of a head are one
+            // run of bytes, copied in one piece; the three warps start the copies in turn); the
+            // warps turn each into a 16-bit tile, 16 dims of a key at a time.
+            constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
+            const uint32_t i0 = threadIdx.x - 9 * 32;
+            const uint32_t in_page = (1u << p.page_shift) - 1;
+            uint32_t ring = 0, units = 0;
+            bool ok = true;
+            uint32_t u = blockIdx.x;
+            for (uint32_t iter = 0; ok; ++iter) {
+                if (iter && !next_unit(iter - 1, u)) break;
+                const Unit w = unit_at(p, n, u);
+                if (!w.blocks) {
+                    if (!iter) break;  // a block whose first unit is empty leaves
                     if (i0 == 0) ok = ask(iter);
                     ok = __shfl_sync(0xffffffffu, ok, 0);
-                    if (!ok) break;
+                    continue;
                 }
-                __syncwarp();
-                if (i + L::kRaw < count && (i + L::kRaw) % kConverters == turn_of) ok = fetch(i + L::kRaw);
+                // lanes 0 to 7 have the page of their piece of a block
+                const uint32_t piece = min(1u << p.page_shift, kKeys);
+                auto page_of = [&](uint32_t j) -> int32_t {
+                    const uint32_t in_block = lane * piece, key = (w.first + j) * kKeys + in_block;
+                    if (in_block >= kKeys || key >= w.len) return -1;
+                    const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
+                    if (page < 0 || (uint32_t)page >= p.pages) {
+                        atomicExch(p.err, 3);
+                        return -1;
+                    }
+                    return page;
+                };
+                const uint32_t count = 2 * w.blocks, turn_of = i0 / 32;
+                int32_t page_next = turn_of < count ? page_of(turn_of / 2) : -1;  // for the warp's next tile
+                // Starts the copies of tile i (K_j: 2j, V_j: 2j + 1). Keys of no page, and past the
+                // end, keep what the slot holds: any byte is a finite code, and they weigh nothing.
+                auto fetch = [&](uint32_t i) -> bool {
+                    const uint32_t at = ring + i, slot = at % L::kRaw;
+                    if (!warp_wait(&raw_empty[slot], (at / L::kRaw) ^ 1u)) return false;
+                    const int32_t page_now = page_next;
+                    if (i + kConverters < count) page_next = page_of((i + kConverters) / 2);
+                    const uint32_t bytes = piece * p.head_dim;
+                    const uint32_t live = __popc(__ballot_sync(0xffffffffu, page_now >= 0));
+                    if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], live * bytes);
+                    __syncwarp();
+                    if (page_now >= 0) {
+                        const uint32_t key = (w.first + i / 2) * kKeys + lane * piece;
+                        const int8_t* from =
+                            static_cast<const int8_t*>(i & 1 ? p.v : p.k) +
+                            ((((uint64_t)page_now * p.kv_heads + w.kv_head) << p.page_shift) + (key & in_page)) * p.head_dim;
+                        asm volatile(
+                            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                                smem_addr(sRaw + slot * L::kRawBytes + lane * bytes)),
+                            "l"(from), "r"(bytes), "r"(smem_addr(&raw_full[slot]))
+                            : "memory");
+                    }
+                    __syncwarp();
+                    return true;
+                };
+                for (uint32_t i = turn_of; ok && i < min(count, L::kRaw); i += kConverters) ok = fetch(i);
+                if (!ok) break;
+                // the largest V scale of the keys in reach. The ring's tiles are those of at most
+                // three units, so that the slot's last value has been read.
+                if (turn_of == 0) {
+                    float top = 1e-30f;
+                    const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
+#pragma unroll 4
+                    for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
+                        const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
+                        if (page >= 0 && (uint32_t)page < p.pages)
+                            top = fmaxf(top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
+                    }
+                    top = warp_max(top);
+                    if (lane == 0) {
+                        s_top[units & 3u] = top;
+                        mbar_arrive(&top_full[units & 3u]);
+                    }
+                    __syncwarp();
+                }
+                ++units;
+                for (uint32_t i = 0; ok && i < count; ++i) {
+                    const uint32_t at = ring + i, st = at % kStages, slot = at % L::kRaw;
+                    ok = warp_wait(&raw_full[slot], at / L::kRaw) && warp_wait(&empty[st], (at / kStages) ^ 1u);
+                    if (!ok) break;
+                    uint8_t* to = sKV + st * L::kOperand;
+                    const uint8_t* from = sRaw + slot * L::kRawBytes;
+                    // a batch of loads ahead of its conversions and stores, which the compiler keeps in the
+                    // order written (one by one: 143 us for 134)
+                    constexpr uint32_t kPieces = (kKeys * kParts + kStep - 1) / kStep, kBatch = 4;
+#pragma unroll
+                    for (uint32_t k0 = 0; k0 < kPieces; k0 += kBatch) {
+                        uint4 x[kBatch];
+                        uint32_t key[kBatch], part[kBatch];
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            // eight lanes: four dims' parts of two rows, at D = 128 the first half of one and
+                            // the second of the other, which spreads loads and stores over the banks
+                            const uint32_t at16 = i0 + kStep * (k0 + k);
+                            key[k] = D == 64 ? at16 / 4 : at16 / 16 * 2 + (at16 / 4 & 1);
+                            part[k] = D == 64 ? at16 % 4 : at16 % 4 + 4 * ((at16 / 4 ^ at16 / 8) & 1);
+                            x[k] = make_uint4(0, 0, 0, 0);
+                            if (key[k] < kKeys && 16 * part[k] < p.head_dim)
+                                x[k] = *reinterpret_cast<const uint4*>(from + key[k] * p.head_dim + 16 * part[k]);
+                        }
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            if (key[k] >= kKeys) continue;
+                            const uint32_t w4[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u,
+                                                    x[k].w ^ 0x80808080u};
+                            *reinterpret_cast<uint4*>(to + chunk_at(key[k], 2 * part[k])) =
+                                make_uint4(codes_lo(w4[0]), codes_hi(w4[0]), codes_lo(w4[1]), codes_hi(w4[1]));
+                            *reinterpret_cast<uint4*>(to + chunk_at(key[k], 2 * part[k] + 1)) =
+                                make_uint4(codes_lo(w4[2]), codes_hi(w4[2]), codes_lo(w4[3]), codes_hi(w4[3]));
+                        }
+                    }
+                    fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&full[st]);
+                        mbar_arrive(&raw_empty[slot]);
+                    }
+                    if (i == min(4u, count - 1)) {
+                        if (i0 == 0) ok = ask(iter);
+                        ok = __shfl_sync(0xffffffffu, ok, 0);
+                        if (!ok) break;
+                    }
+                    __syncwarp();
+                    if (i + L::kRaw < count && (i + L::kRaw) % kConverters == turn_of) ok = fetch(i + L::kRaw);
+                }
+                ring += count;
             }
-            ring += count;
         }
     }
 
@@ -975,8 +1016,8 @@ bool encode_queries(CUtensorMap& tm, const RowsParams& p, uint32_t tokens, bool 
 }
 
 template <int D, bool kS8, bool kBF16>
-int start(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, const TilesParams& n, uint32_t units,
-          cudaStream_t st) {
+int start(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const RowsParams& p, const TilesParams& n,
+          uint32_t blocks, cudaStream_t st) {
     using L = Layout<D, kS8>;
     auto kernel = attention_tiles_kernel<D, kS8, kBF16>;
     static std::atomic<uint64_t> configured;  // one bit per device ordinal
@@ -989,7 +1030,7 @@ int start(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, cons
             return set_error(DAV2CUDA_LAUNCH_FAILED, "attention: cannot set shared memory size");
         mark_configured(configured, dev);
     }
-    kernel<<<units, kThreads, L::kSmem, st>>>(q, k, v, p, n);
+    kernel<<<blocks, kThreads, L::kSmem, st>>>(q, k, v, p, n);
     return check_launch("attention_tiles");
 }
 
@@ -1024,9 +1065,10 @@ int launch_attention_tiles(const RowsParams& p, uint32_t slots, bool s8, bool bf
     cudaGetDevice(&dev);
     n.takes_over = units > (uint64_t)sm_count(dev);
     const bool small = p.head_dim <= 64;
-    if (s8) return small ? start<64, true, false>(q, k, v, p, n, (uint32_t)units, st) : start<128, true, false>(q, k, v, p, n, (uint32_t)units, st);
-    if (bf16) return small ? start<64, false, true>(q, k, v, p, n, (uint32_t)units, st) : start<128, false, true>(q, k, v, p, n, (uint32_t)units, st);
-    return small ? start<64, false, false>(q, k, v, p, n, (uint32_t)units, st) : start<128, false, false>(q, k, v, p, n, (uint32_t)units, st);
+    const uint32_t blocks = (uint32_t)units;
+    if (s8) return small ? start<64, true, false>(q, k, v, p, n, blocks, st) : start<128, true, false>(q, k, v, p, n, blocks, st);
+    if (bf16) return small ? start<64, false, true>(q, k, v, p, n, blocks, st) : start<128, false, true>(q, k, v, p, n, blocks, st);
+    return small ? start<64, false, false>(q, k, v, p, n, blocks, st) : start<128, false, false>(q, k, v, p, n, blocks, st);
 }
 
 }  // namespace dav2cuda

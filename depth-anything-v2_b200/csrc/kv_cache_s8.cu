@@ -9,10 +9,13 @@
 // ratio rounded to f32. Infinities take the codes +-127 and NaN the code 0, and
 // neither enters a scale.
 //
-// Bound by memory: the rows are read once, into registers, and the codes written once. One block for each page that receives tokens, each head, and K or
-// V; the blocks of sequence s are numbered from floor(begin[s] / page_tokens) + 2 s,
-// which leaves room for its pages whatever their boundaries, so that the host
-// needs no length: blocks without a page leave at once.
+// Bound by memory: the rows are read once, into registers, and the codes written once
+// (20011 tokens of 5 prompts, 8 heads of 128, f16: 34 us, 3.7 TB/s; what is missing to the
+// memory's rate is each block's own chain from its offsets over its page to its rows). One
+// block for each page that receives tokens, each head, and K or V; the blocks of sequence s
+// are numbered from floor(begin[s] / page_tokens) + 2 s, which leaves room for its pages
+// whatever their boundaries, so that the host needs no length: blocks without a page leave
+// at once.
 #include <type_traits>
 
 #include "abi_check.h"
@@ -243,7 +246,7 @@ extern "C" DAV2CUDA_API int dav2cuda_kv_cache_append_s8(
     DAV2_REQUIRE(blocks <= 0x7FFFFFFFu, "cache append: too many tokens or sequences");
     const cudaStream_t st = as_stream(stream);
     // a few tokens for each sequence are the work of few threads, and blocks of few threads all
-    // fit the SMs at once (64 sequences, one token each: STEP us)
+    // fit the SMs at once (64 sequences, one token each: 5.7 us, with 128 threads 7.4)
     if (tokens <= 4ull * sequences) start<64>(p, (uint32_t)blocks, precision, st);
     else start<128>(p, (uint32_t)blocks, precision, st);
     return check_launch("kv_cache_append_s8");

@@ -413,7 +413,12 @@ DAV2CUDA_API uint64_t dav2cuda_attention_head64_workspace_size(uint32_t batch, u
  * after another), so that a part of a packed q|k|v row can be passed in place.
  * Device arrays of lengths, offsets and pages are read by the kernels; a value
  * out of range is never used as an address: the work that it belongs to is left
- * out (a length is clamped) and the device error word becomes 3. */
+ * out (a length is clamped) and the device error word becomes 3; what the rows
+ * concerned then hold is undefined.
+ *
+ * Outputs overlap no input, unless an entry says so. A workspace belongs to one
+ * call at a time: calls that may run at once (on several streams, in several
+ * graphs) need one each. Without need of one (size 0) it may be NULL. */
 
 /* Rotary frequencies, computed on the host: frequency j of each axis =
  * base^(-j / count), count = rotary_dim / 2 / axes, host_frequencies
@@ -465,7 +470,8 @@ DAV2CUDA_API int dav2cuda_qk_norm_rope(void* q_output, void* k_output, const voi
  * codes +-127 and NaN the code 0; neither enters a scale. Places behind the last
  * token stay as they were. page_tokens 16, 32, 64 or 128, head_dim a multiple of
  * 16 up to 128. A page that receives rows may belong to one sequence only;
- * sequences may share full pages. 16-byte aligned rows and codes. */
+ * sequences may share full pages. Scales are 0 or more. 16-byte aligned rows and
+ * codes. */
 DAV2CUDA_API int dav2cuda_kv_cache_append_s8(int8_t* k_codes, float* k_scales, int8_t* v_codes,
                                              float* v_scales, const void* k, const void* v,
                                              const int32_t* page_table, const int32_t* cached,
@@ -480,8 +486,10 @@ DAV2CUDA_API int dav2cuda_kv_cache_append_s8(int8_t* k_codes, float* k_scales, i
  * [head_dim], bf16 or f16) and lengths[s] <= max_length tokens in the cache, the
  * new ones included. causal != 0: its queries are its last tokens, query i of n
  * sees the first lengths[s] - n + i + 1 tokens. Query head h reads key head
- * h / (q_heads / kv_heads). A query that sees nothing gives zeros; rows of no
- * sequence stay as they were. Output f32 or of q's type. Products with f16
+ * h / (q_heads / kv_heads). A query that sees nothing, or nothing but scores of
+ * -inf, gives zeros; one with a score of inf or NaN gives NaN; rows of no
+ * sequence stay as they were. head_dim a multiple of 16 up to 128; 16-byte
+ * aligned rows and codes; scales 0 or more. Output f32 or of q's type. Products with f16
  * operands (codes exactly, q scaled by a power of two, softmax weights rounded
  * to f16) and f32 accumulation. workspace_size answers for the same numbers. */
 DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint32_t sequences, uint32_t queries,
@@ -502,7 +510,8 @@ DAV2CUDA_API int dav2cuda_attention_cache_s8(void* output, const void* q, const 
 /* Attention of q [batch][queries][q_heads][head_dim] to k and v [batch][keys]
  * [kv_heads][head_dim], bf16 or f16: softmax(scale * q . k) . v over the first
  * key_lengths[b] keys (key_lengths NULL: all). Keys behind that are not read
- * into the result, whatever they hold; a batch entry without keys gives zeros.
+ * into the result, whatever they hold; a batch entry without keys, or a row with
+ * nothing but scores of -inf, gives zeros, a row with a score of inf or NaN NaN.
  * head_dim a multiple of 8 up to 128; 16-byte aligned rows; batch and token
  * strides as given. Query head h reads key head h / (q_heads / kv_heads). Output
  * f32 or of the operands' type. f32 accumulation, softmax weights rounded to the
