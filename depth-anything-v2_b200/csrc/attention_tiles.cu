@@ -36,7 +36,7 @@
 // 128 alike (0.8 with the polynomials), the products 0.65 and 1.1 us, and each tile's chain from
 // its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
 // other's alone.
-// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 138 us (446 TFLOP/s); 4 x 1370 x 5477, 16
+// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 134 us (459 TFLOP/s); 4 x 1370 x 5477, 16
 // heads of 128 on 4 key heads, padded batch, 216 us (890 TFLOP/s). Codes: the chain of one
 // issuer and the conversion on top; 700 queries over 6 caches of up to 6000 tokens, 32 heads
 // of 128 on 8 key heads, 134 us (298 TFLOP/s).
@@ -511,19 +511,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 a[0] = fmax3(a[0], s[124], s[125]), a[1] = fmax3(a[1], s[126], s[127]);
                 float top = fmax3(fmax3(a[0], a[1], a[2]), a[3], a[3]);
                 if constexpr (!kS8) top = top == -INFINITY ? top : top * c;
-                if constexpr (!L::kAlias) {
-                    // P's columns, and O: the product of the block before is done
-                    if (j > 0 && !warp_wait(&pv_done[t], done - 1)) {
-                        ok = false;
-                        break;
-                    }
+                // P's columns, and O, are free once the product of the block before is done: waited for
+                // where they are written (before the maximum's vote: 138 us for 134)
+                auto last_product = [&]() -> bool {
+                    const bool done_now = warp_wait(&pv_done[t], done - 1);
                     tc_fence_after();
-                }
+                    return done_now;
+                };
                 const bool raise = top > m + kRaise;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float up = fmaxf(m, top);
                     const float down = ex2_approx(m - up);
                     if (j > 0) {  // with P in S's columns, P V was issued before this S
+                        if (!L::kAlias) ok = last_product();
 #pragma unroll 1
                         for (uint32_t k = 0; k < D / 8; ++k) {
                             uint32_t o[8];
@@ -559,8 +559,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if constexpr (kS8) f2_mul(x, y, x, y, sv[i / 8], sv[i / 8]);
                         x2[i] = pack2<kBF16>(x, y);
                     }
+                    if (!L::kAlias && h == 0 && j > 0) ok = last_product() && ok;
                     tmem_st_32x32b_x32(tP + 32u * h, x2);
                 }
+                if (!ok) break;
                 l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                 if (top != top) l = top;  // a score is NaN: emulated exponentials would lose it
                 tmem_st_wait();
