@@ -37,7 +37,7 @@
 // its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
 // other's alone.
 // Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 134 us (459 TFLOP/s); 4 x 1370 x 5477, 16
-// heads of 128 on 4 key heads, padded batch, 216 us (890 TFLOP/s). Codes: the chain of one
+// heads of 128 on 4 key heads, padded batch, 220 us (873 TFLOP/s). Codes: the chain of one
 // issuer and the conversion on top; 700 queries over 6 caches of up to 6000 tokens, 32 heads
 // of 128 on 8 key heads, 134 us (298 TFLOP/s).
 // Every wait is bounded (kWaitTimeoutNs); a timeout sets the device error word.
