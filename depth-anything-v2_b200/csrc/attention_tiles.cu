@@ -36,7 +36,7 @@
 // 128 alike (0.8 with the polynomials), the products 0.65 and 1.1 us, and each tile's chain from
 // its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
 // other's alone.
-// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 134 us (459 TFLOP/s); 4 x 1370 x 5477, 16
+// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 129 us (477 TFLOP/s); 4 x 1370 x 5477, 16
 // heads of 128 on 4 key heads, padded batch, 220 us (873 TFLOP/s). Codes: the chain of one
 // issuer and the conversion on top; 700 queries over 6 caches of up to 6000 tokens, 32 heads
 // of 128 on 8 key heads, 134 us (298 TFLOP/s).
@@ -154,6 +154,19 @@ __device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
+}
+
+// 32 bytes of a row that starts on a 16-byte boundary: in one piece where they lie so. A lane
+// has a row of its own, and what its stores cost is their number (131 us for 129).
+__device__ __forceinline__ void store32(void* to, const uint32_t (&x)[8]) {
+    if ((reinterpret_cast<uintptr_t>(to) & 31u) == 0) {
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(to), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+                     "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+                     : "memory");
+    } else {
+        reinterpret_cast<uint4*>(to)[0] = make_uint4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<uint4*>(to)[1] = make_uint4(x[4], x[5], x[6], x[7]);
+    }
 }
 
 // The largest of three; NaN if one is.
@@ -380,9 +393,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t units = 0;  // units with keys so far
         bool ok = true;
         uint32_t u = blockIdx.x;
+        Unit next = unit_at(p, n, u);
+        bool more = true, looked = true;  // of the next unit, found while the last product runs
         for (uint32_t iter = 0;; ++iter) {
-            if (iter && !next_unit(iter - 1, u)) break;
-            const Unit w = unit_at(p, n, u);
+            if (!looked) {
+                more = next_unit(iter - 1, u);
+                if (more) next = unit_at(p, n, u);
+            }
+            if (!more) break;
+            looked = false;
+            const Unit w = next;
             if (!w.any) {
                 if (!iter) break;
                 continue;
@@ -570,7 +590,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
-            if (!ok || !warp_wait(&o_full[t], outs++)) break;
+            if (!ok) break;
+            more = next_unit(iter, u);
+            if (more) next = unit_at(p, n, u);
+            looked = true;
+            if (!warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
             if (m == kLowest) l = 0.0f;  // a row that sees nothing: its P is 0 or, emulated, 2^-126
             if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
@@ -585,24 +609,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tmem_ld_wait();
                 if (!live) continue;
 #pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    if (32 * k + i >= p.head_dim) continue;
-                    float x[8];
+                for (int i = 0; i < 32; i += 16) {
+                    const uint32_t dim = 32 * k + i;
+                    if (dim >= p.head_dim) continue;
+                    const bool whole = dim + 16 <= p.head_dim;  // else 8 dims
+                    float x[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = l != 0.0f ? __uint_as_float(o[i + e]) * f : 0.0f;
+                    for (int e = 0; e < 16; ++e) x[e] = l != 0.0f ? __uint_as_float(o[i + e]) * f : 0.0f;
+                    uint32_t y[8];
                     if (p.splits > 1 || p.out_kind == 0) {
-                        float* to = p.splits > 1 ? p.part_o + at * p.head_dim : static_cast<float*>(p.out) + at;
-                        float4* to4 = reinterpret_cast<float4*>(to + 32 * k + i);
-                        to4[0] = make_float4(x[0], x[1], x[2], x[3]);
-                        to4[1] = make_float4(x[4], x[5], x[6], x[7]);
-                    } else {
-                        uint32_t y[4];
+                        float* to = (p.splits > 1 ? p.part_o + at * p.head_dim : static_cast<float*>(p.out) + at) + dim;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
+                        for (int h = 0; h < 2; ++h) {
+                            if (h && !whole) continue;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[e] = __float_as_uint(x[8 * h + e]);
+                            store32(to + 8 * h, y);
+                        }
+                    } else {
+                        uint16_t* to = static_cast<uint16_t*>(p.out) + at + dim;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
                             y[e] = p.out_kind == 1 ? pack2<true>(x[2 * e], x[2 * e + 1])
                                                    : pack2<false>(x[2 * e], x[2 * e + 1]);
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + 32 * k + i) =
-                            make_uint4(y[0], y[1], y[2], y[3]);
+                        if (whole) store32(to, y);
+                        else *reinterpret_cast<uint4*>(to) = make_uint4(y[0], y[1], y[2], y[3]);
                     }
                 }
             }
