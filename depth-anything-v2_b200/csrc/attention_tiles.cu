@@ -596,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             looked = true;
             if (!warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
-            if (m == kLowest) l = 0.0f;  // a row that sees nothing: its P is 0 or, emulated, 2^-126
+            // a row that sees nothing: its P is 0 or, emulated, 2^-126. NaN, which raises no maximum, stays
+            if (m == kLowest && l == l) l = 0.0f;
             if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
             const float unit_v = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
             const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
