@@ -22,13 +22,13 @@
 // Codes become f16 exactly (byte + 1024 by a byte permutation, minus 1152), and q
 // is scaled by a power of two for each row into f16's range, which keeps every
 // bit of a bf16 or f16 value within 2^-29 of the row's largest. A K scale multiplies the
-// scores of its 16 keys; a V scale multiplies p before it is rounded to f16,
-// relative to the largest V scale R that the warp has met (O is kept in units of
-// R and rescaled when R grows). p is at most 2^8 (m follows the row's maximum
-// only when that exceeds it by 8) and is kept times 2^7, so that f16 holds
-// contributions down to 2^-31 of the largest. The sum of p is kept in f32 from
-// the unrounded values. 16-bit values take p in their own type, as the tensor
-// core wants both operands alike.
+// scores of its 16 keys; a V scale 2^e f adds e to them and multiplies p by f before it
+// is rounded to f16, so that m is the maximum of score + e: of what keys contribute, not
+// of their scores alone. p is at most 2^7 (m follows the row's maximum only when that
+// exceeds it by 7) and is kept times 2^7, so that f16 holds contributions down to 2^-31
+// of the row's largest, whatever the scales of pages that it does not see or gives no
+// weight. The sum takes p times 2^-e in f32, unrounded. 16-bit values take p in their own
+// type, as the tensor core wants both operands alike (p at most 2^8).
 //
 // A block's four warps take the same rows and every fourth step of keys, or (more than 16
 // rows) two row tiles and every second step, merged at the end in shared memory. Where
@@ -52,7 +52,9 @@ namespace {
 
 constexpr uint32_t kWarps = 4;
 constexpr uint32_t kThreads = 32 * kWarps;
-constexpr float kRaise = 8.0f;    // m is raised when a score exceeds it by this
+// m is raised when a score exceeds it by this: p times a scale's f < 2 and 2^7 stays in f16
+template <bool kS8>
+constexpr float kRaise = kS8 ? 7.0f : 8.0f;
 // Where m starts: finite, so that -inf - m is -inf and rows that see nothing get p = 0
 // without a test; any finite score above it raises it.
 constexpr float kLowest = -3.402823466e38f;
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     }
     const uint32_t last = min(min(chunks, first + per_split), (high + kChunk - 1) / kChunk);
 
-    float o[kSteps][NT][4], m[NT][2], l[NT][2], ref = 1e-30f, inv_ref = 128.0f / 1e-30f;
+    float o[kSteps][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -344,18 +346,20 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             step_in = step_in + 1 == Keys::kSteps ? 0 : step_in + 1;
         }
         const uint32_t from = f.base + step * Keys::kStep;
-        float sk[kTiles], sv[kTiles], sv_top = 0.0f;
+        float sk[kTiles], shift[kTiles], weight[kTiles], back_v[kTiles];  // V scale: 2^shift, f times 2^7, 2^-shift
         bool any_dead = false;
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
-            sk[b] = sv[b] = 1.0f;
+            sk[b] = 1.0f;
             if constexpr (kS8) {
+                float sv;
                 const uint32_t at = f.scales + step * 16 + 4 * b;
                 asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sk[b]) : "r"(at) : "memory");
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sv[b]) : "r"(at + 4 * kTiles) : "memory");
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(sv) : "r"(at + 4 * kTiles) : "memory");
                 any_dead |= sk[b] < 0.0f;
+                split_scale(sv, shift[b], weight[b], back_v[b]);
+                weight[b] *= 128.0f;
             }
-            sv_top = fmaxf(sv_top, sv[b]);
         }
         step = step + 1 == Keys::kSteps ? 0 : step + 1;
         float sc[kTiles][NT][4];
@@ -393,7 +397,10 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[b][n][e] *= kS8 ? factor[n][e & 1] * sk[b] : factor[n][e & 1];
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (kS8) sc[b][n][e] = fmaf(sc[b][n][e], factor[n][e & 1] * sk[b], shift[b]);
+                    else sc[b][n][e] *= factor[n][e & 1];
+                }
         if (key0 + kChunk > low || any_dead) {
             const uint32_t key = key0 + 4 * (g >> 1) + (g & 1);
 #pragma unroll
@@ -411,15 +418,9 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             for (int e = 0; e < 2; ++e) {
                 top[n][e] = fmaxf(sc[0][n][e], sc[0][n][e + 2]);
                 if (kTiles == 2) top[n][e] = fmaxf(top[n][e], fmaxf(sc[kTiles - 1][n][e], sc[kTiles - 1][n][e + 2]));
-                raise |= top[n][e] > m[n][e] + kRaise;
+                raise |= top[n][e] > m[n][e] + kRaise<kS8>;
             }
-        if (__any_sync(0xffffffffu, raise) || (kS8 && sv_top > ref)) {
-            float unit = 1.0f;
-            if (kS8 && sv_top > ref) {
-                unit = ref / sv_top;
-                ref = sv_top;
-                inv_ref = 128.0f / ref;
-            }
+        if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -432,22 +433,25 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
                     m[n][e] = x;
                     l[n][e] *= down;
 #pragma unroll
-                    for (int i = 0; i < kSteps; ++i) o[i][n][e] *= down * unit, o[i][n][e + 2] *= down * unit;
+                    for (int i = 0; i < kSteps; ++i) o[i][n][e] *= down, o[i][n][e + 2] *= down;
                 }
         }
         uint32_t pf[kTiles][NT][2];
 #pragma unroll
         for (int b = 0; b < kTiles; ++b) {
-            const float weight = kS8 ? sv[b] * inv_ref : kBF16 ? 1.0f : 128.0f;
+            const float w = kS8 ? weight[b] : kBF16 ? 1.0f : 128.0f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float e4[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) e4[e] = ex2_approx(sc[b][n][e] - m[n][e & 1]);
-                l[n][0] += e4[0] + e4[2];
-                l[n][1] += e4[1] + e4[3];
-                pf[b][n][0] = transpose8x8(pack2<kBF16>(e4[0] * weight, e4[1] * weight));
-                pf[b][n][1] = transpose8x8(pack2<kBF16>(e4[2] * weight, e4[3] * weight));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (kS8) l[n][e] = fmaf(e4[e] + e4[e + 2], back_v[b], l[n][e]);
+                    else l[n][e] += e4[e] + e4[e + 2];
+                }
+                pf[b][n][0] = transpose8x8(pack2<kBF16>(e4[0] * w, e4[1] * w));
+                pf[b][n][1] = transpose8x8(pack2<kBF16>(e4[2] * w, e4[3] * w));
             }
         }
 #pragma unroll
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
     __syncthreads();
 
     // this warp's result: sums over the lanes that share a column, O in true units
-    const float unit = kS8 ? ref * (1.0f / 128.0f) : kBF16 ? 1.0f : 1.0f / 128.0f;
+    const float unit = kBF16 ? 1.0f : 1.0f / 128.0f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -39,6 +39,18 @@ __device__ __forceinline__ uint32_t hsub2_1152(uint32_t x) {
 __device__ __forceinline__ uint32_t codes_lo(uint32_t x) { return hsub2_1152(prmt(x, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t codes_hi(uint32_t x) { return hsub2_1152(prmt(x, 0x64646464u, 0x4342)); }
 
+// The V scale of a page as 2^e f, f in [1, 2). 2^e is added to the exponent of its keys, so that the
+// running maximum, and what f16 holds of the weights, goes by p 2^e of the keys that the row itself
+// sees: neither a page behind its mask nor one that it gives no weight takes bits from the others,
+// however large its scale. f multiplies the weight, back = 2^-e brings it to p for the sum; all exact.
+// Scales below 2^-90 leave the rest in f, which keeps 2^(7 - e) times 2^31 keys within f32.
+__device__ __forceinline__ void split_scale(float scale, float& e, float& f, float& back) {
+    const int i = max(-90, min(126, (int)(__float_as_uint(scale) >> 23) - 127));
+    e = (float)i;
+    back = __uint_as_float((uint32_t)(127 - i) << 23);
+    f = scale * back;
+}
+
 template <bool kBF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (kBF16) {

@@ -29,8 +29,9 @@
 //
 // Keys past the end: scores are replaced by -inf; the rows of V behind the last
 // key are set to zero in shared memory before the last product, as they may hold
-// NaN. Codes: K's scale multiplies the scores of its page's keys, V's scale, over
-// the largest of the sequence, multiplies P before it is rounded.
+// NaN. Codes: K's scale multiplies the scores of its page's keys; V's scale 2^e f adds
+// e to them and multiplies P by f before it is rounded, and the sum takes P times 2^-e, so
+// that P's range is that of what the row's keys contribute (attention_rows.cuh).
 //
 // Bound by the softmax: for 128 keys an SM's four exponential units need 1.1 us at D = 64 and
 // 128 alike (0.8 with the polynomials), the products 0.65 and 1.1 us, and each tile's chain from
@@ -55,7 +56,9 @@ namespace {
 constexpr uint32_t kTileRows = 128;
 constexpr uint32_t kKeys = 128;        // keys of a block
 constexpr uint32_t kAtom = 128 * 128;  // bytes of 128 rows x 64 dims of 16 bits
-constexpr float kRaise = 8.0f;
+// P is at most 2^8; codes: 2^7, times f < 2 and 2^7 in f16
+template <bool kS8>
+constexpr float kRaise = kS8 ? 7.0f : 8.0f;
 constexpr uint32_t kSoftmaxWarps = 8;
 constexpr uint32_t kConverters = 3;     // codes
 constexpr uint32_t kThreads = 12 * 32;  // 168 registers each at launch
@@ -302,13 +305,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t* unit_empty = unit_full + 2;  // [response]
     uint64_t* turn = unit_empty + 2;     // [tile]
     uint64_t* drain = turn + 2;
-    uint64_t* top_full = drain + 2;      // codes: [unit % 4]
-    uint64_t* raw_full = top_full + 4;   // [raw slot]
-    uint64_t* raw_empty = raw_full + 4;  // [raw slot]
+    uint64_t* raw_full = drain + 2;      // codes: [raw slot]
+    uint64_t* raw_empty = raw_full + 4;  // codes: [raw slot]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 4);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    float* s_top = reinterpret_cast<float*>(tmem_slot + 4);  // codes: [unit % 4] the largest V scale
-    static_assert(32 + 8 * (2 * kStages + 34) + 32 <= L::kBars, "barriers overflow their part");
+    static_assert(32 + 8 * (2 * kStages + 30) + 32 <= L::kBars, "barriers overflow their part");
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if ((smem_addr(smem) & 1023u) != 0) {  // the 128-byte swizzle needs 1 KB aligned tiles
@@ -333,7 +334,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&unit_empty[t], kSoftmaxWarps + kIssuers<D, kS8> + (kS8 ? kConverters : 2));  // warps at work
         }
         for (uint32_t i = 0; kS8 && i < 4; ++i) {
-            mbar_init(&top_full[i], 1);
             mbar_init(&raw_full[i], 1);
             mbar_init(&raw_empty[i], kConverters);
         }
@@ -390,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tO = tmem + L::kO + t * D + lanes;
         uint32_t done = 0;   // blocks of this tile so far
         uint32_t outs = 0;   // units of this tile so far
-        uint32_t units = 0;  // units with keys so far
         bool ok = true;
         uint32_t u = blockIdx.x;
         Unit next = unit_at(p, n, u);
@@ -422,10 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!iter) break;
                 continue;
             }
-            const uint32_t unit = units++;
             if (t >= w.tiles) continue;
             // a negative scale is in the first product's sign; above 0, so that the -inf of a masked key stays
-            float c = fmaxf(fabsf(p.scale_log2), 1e-35f), v_top = 1.0f;
+            float c = fmaxf(fabsf(p.scale_log2), 1e-35f);
             if constexpr (kS8) {
                 // this row of Q, brought into f16's range by a power of two. The last unit's
                 // products are done: this warp has waited for its output.
@@ -456,8 +454,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[t]);
-                if (!warp_wait(&top_full[unit & 3u], unit >> 2)) break;
-                v_top = s_top[unit & 3u];
             }
             // where the row's result goes, found now: the unit's numbers need no registers later
             const uint64_t at = !live ? 0
@@ -465,17 +461,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                : row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
             const uint32_t reach = reach_of(p, w.where, w.len, row);
             const uint32_t low = __reduce_min_sync(0xffffffffu, live ? reach : 0xFFFFFFFFu);
-            // codes: lane i has the K scale (i < 8), lane 8 + i the V scale over the largest,
-            // of the block's keys 16i .. 16i + 15; fetched a block ahead. -1: no such page
+            // codes: lane i has the K scale (i < 8), lane 8 + i the V scale, of the block's keys
+            // 16i .. 16i + 15; fetched a block ahead. -1: no such page
             auto scale_of = [&](uint32_t j) -> float {
                 const uint32_t key = (w.first + j) * kKeys + 16u * (lane & 7u);
                 if (lane >= 16 || key >= w.len) return 0.0f;
                 const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + (key >> p.page_shift)];
                 if (page < 0 || (uint32_t)page >= p.pages) return lane < 8 ? -1.0f : 0.0f;
                 const uint64_t unit = (uint64_t)page * p.kv_heads + w.kv_head;
-                return lane < 8 ? p.k_scales[unit] : p.v_scales[unit] * (128.0f / v_top);
+                return (lane < 8 ? p.k_scales : p.v_scales)[unit];
             };
-            float scale_next = 0.0f, scale_now = 0.0f;
+            float scale_next = 0.0f, scale_now = 0.0f, v_shift = 0.0f, v_weight = 0.0f, v_back = 0.0f;
             if constexpr (kS8) scale_next = scale_of(0);
             float m = kLowest, l = 0.0f;
             // f16: P is kept times 2^7, which leaves f16 down to 2^-31 of the row's largest
@@ -502,11 +498,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (kS8) {
                     scale_now = scale_next;
                     if (j + 1 < w.blocks) scale_next = scale_of(j + 1);
+                    split_scale(fmaxf(scale_now, 0.0f), v_shift, v_weight, v_back);  // lanes 8 to 15
+                    v_weight *= 128.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const float f = __shfl_sync(0xffffffffu, scale_now, i) * c;
+                        const float shift = __shfl_sync(0xffffffffu, v_shift, 8 + i);
 #pragma unroll
-                        for (int e = 16 * i; e < 16 * i + 16; e += 2) f2_mul(s[e], s[e + 1], s[e], s[e + 1], f, f);
+                        for (int e = 16 * i; e < 16 * i + 16; e += 2)
+                            f2_fma(s[e], s[e + 1], s[e], s[e + 1], f, f, shift, shift);
                     }
                     if (__any_sync(0xffffffffu, scale_now < 0.0f)) {  // keys of no page of the cache
 #pragma unroll
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_after();
                     return done_now;
                 };
-                const bool raise = top > m + kRaise;
+                const bool raise = top > m + kRaise<kS8>;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float up = fmaxf(m, top);
                     const float down = ex2_approx(m - up);
@@ -563,11 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint32_t x2[32];
-                    float sv[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-                    if constexpr (kS8) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) sv[i] = __shfl_sync(0xffffffffu, scale_now, 8 + 4 * h + i);
-                    }
+                    float part[4];  // codes: sum over the 16 keys of a V scale
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         float x = s[64 * h + 2 * i], y = s[64 * h + 2 * i + 1];
@@ -575,8 +571,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else f2_fma(x, y, x, y, c, c, off, off);
                         if (i % 8 < kEmulated<kS8>) exp2_pair(x, y);
                         else x = ex2_approx(x), y = ex2_approx(y);
-                        f2_add(ls[(2 * i) & 3], ls[(2 * i + 1) & 3], ls[(2 * i) & 3], ls[(2 * i + 1) & 3], x, y);
-                        if constexpr (kS8) f2_mul(x, y, x, y, sv[i / 8], sv[i / 8]);
+                        if constexpr (kS8) {
+                            constexpr int kPairs = 8;
+                            const int e = 2 * (i & 1);
+                            if (i % kPairs < 2) part[e] = x, part[e + 1] = y;
+                            else f2_add(part[e], part[e + 1], part[e], part[e + 1], x, y);
+                            const float weight = __shfl_sync(0xffffffffu, v_weight, 8 + 4 * h + i / kPairs);
+                            f2_mul(x, y, x, y, weight, weight);
+                            if (i % kPairs == kPairs - 1) {
+                                const float back = __shfl_sync(0xffffffffu, v_back, 8 + 4 * h + i / kPairs);
+                                f2_fma(ls[0], ls[1], part[0], part[1], back, back, ls[0], ls[1]);
+                                f2_fma(ls[2], ls[3], part[2], part[3], back, back, ls[2], ls[3]);
+                            }
+                        } else {
+                            f2_add(ls[(2 * i) & 3], ls[(2 * i + 1) & 3], ls[(2 * i) & 3], ls[(2 * i + 1) & 3], x, y);
+                        }
                         x2[i] = pack2<kBF16>(x, y);
                     }
                     if (!L::kAlias && h == 0 && j > 0) ok = last_product() && ok;
@@ -599,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // a row that sees nothing: its P is 0 or, emulated, 2^-126. NaN, which raises no maximum, stays
             if (m == kLowest && l == l) l = 0.0f;
             if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
-            const float unit_v = kS8 ? v_top * (1.0f / 128.0f) : 1.0f;
+            constexpr float unit_v = kS8 ? 1.0f / 128.0f : 1.0f;
             const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
             const float f = l != 0.0f ? (p.splits == 1 ? unit_v / l : unit_v * back) : 0.0f;
             if (live && p.splits > 1) p.part_ml[at] = make_float2(m, l * back);
@@ -867,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             constexpr uint32_t kParts = D / 16, kStep = 32 * kConverters;
             const uint32_t i0 = threadIdx.x - 9 * 32;
             const uint32_t in_page = (1u << p.page_shift) - 1;
-            uint32_t ring = 0, units = 0;
+            uint32_t ring = 0;
             bool ok = true;
             uint32_t u = blockIdx.x;
             for (uint32_t iter = 0; ok; ++iter) {
@@ -920,25 +929,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 for (uint32_t i = turn_of; ok && i < min(count, L::kRaw); i += kConverters) ok = fetch(i);
                 if (!ok) break;
-                // the largest V scale of the keys in reach. The ring's tiles are those of at most
-                // three units, so that the slot's last value has been read.
-                if (turn_of == 0) {
-                    float top = 1e-30f;
-                    const uint32_t page_end = (min(w.len, (w.first + w.blocks) * kKeys) + in_page) >> p.page_shift;
-#pragma unroll 4
-                    for (uint32_t i = ((w.first * kKeys) >> p.page_shift) + lane; i < page_end; i += 32) {
-                        const int32_t page = p.page_table[(uint64_t)w.where.seq * p.table_stride + i];
-                        if (page >= 0 && (uint32_t)page < p.pages)
-                            top = fmaxf(top, p.v_scales[(uint64_t)page * p.kv_heads + w.kv_head]);
-                    }
-                    top = warp_max(top);
-                    if (lane == 0) {
-                        s_top[units & 3u] = top;
-                        mbar_arrive(&top_full[units & 3u]);
-                    }
-                    __syncwarp();
-                }
-                ++units;
                 for (uint32_t i = 0; ok && i < count; ++i) {
                     const uint32_t at = ring + i, st = at % kStages, slot = at % L::kRaw;
                     ok = warp_wait(&raw_full[slot], at / L::kRaw) && warp_wait(&empty[st], (at / kStages) ^ 1u);

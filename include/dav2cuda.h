@@ -490,8 +490,10 @@ DAV2CUDA_API int dav2cuda_kv_cache_append_s8(int8_t* k_codes, float* k_scales, i
  * -inf, gives zeros; one with a score of inf or NaN gives NaN; rows of no
  * sequence stay as they were. head_dim a multiple of 16 up to 128; 16-byte
  * aligned rows and codes; scales 0 or more. Output f32 or of q's type. Products with f16
- * operands (codes exactly, q scaled by a power of two, softmax weights rounded
- * to f16) and f32 accumulation. workspace_size answers for the same numbers. */
+ * operands (codes exactly, q scaled by a power of two, softmax weights times the V
+ * scale rounded to f16, relative to the row's largest: pages that a row does not see,
+ * or gives no weight, cost it nothing) and f32 accumulation. workspace_size answers for
+ * the same numbers. */
 DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint32_t sequences, uint32_t queries,
                                                                  uint32_t max_length, uint32_t q_heads,
                                                                  uint32_t kv_heads, uint32_t head_dim);

@@ -47,3 +47,46 @@ def test_cache_attention_rows_of_nan(cuda, dav2lib, queries, length, d, p):
     keep = torch.ones_like(out, dtype=torch.bool)
     keep[-1, 1] = False
     assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
+
+
+@pytest.mark.parametrize("up", [20, 40, 110])
+@pytest.mark.parametrize("queries,length,page", [(2, 161, 16), (2, 2945, 64), (100, 161, 16), (100, 3009, 64), (300, 385, 128)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cache_attention_large_values_behind_the_mask(cuda, dav2lib, queries, length, page, d, up):
+    """The last token's page has V scales 2^up times the others': rows that do not see it are as without it."""
+    g = gen(32)
+    c = Cache(g, [length], 2, d, page)
+    begin = [0, queries]
+    q = randn(g, queries, 4, d, dtype=torch.bfloat16)
+    seen = max(0, (length - 1) // page * page - length + queries)  # rows that see earlier pages only
+    assert seen
+    want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, [length], begin, 0.125, True, 0)
+    c.vs[c.table[0][(length - 1) // page]] *= 2.0 ** up
+    out = torch.empty(queries, 4, d, device="cuda")
+    attend_cache(dav2lib, c, q, [length], begin, True, out, 0.125)
+    assert ref.outside(out[:seen], want[:seen], bound[:seen]) <= 1
+    want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, [length], begin, 0.125, True, 0)
+    assert ref.outside(out[seen:], want[seen:], bound[seen:]) <= 1
+
+
+@pytest.mark.parametrize("where", [0, 4, 9])
+@pytest.mark.parametrize("queries", [2, 100])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cache_attention_large_values_without_weight(cuda, dav2lib, queries, d, where):
+    """A page of keys 400 and more below the others in score, with V scales 2^60 times theirs: as without it."""
+    g = gen(33)
+    c = Cache(g, [160], 2, d, 16)
+    c.k[..., 5] = 0
+    q = randn(g, queries, 4, d, dtype=torch.float16)
+    q[..., 5] = 16.0
+    hot = c.table[0][where]
+    pages = [p for p in c.table[0] if p != hot]
+    want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, [pages], [144], [0, queries], 0.125, False, 0)
+    # its scores are 0.125 * 16 * -127 * 2 = -508; the others', of normal q and |k| <= 3.5, are some units from 0
+    c.k[hot] = 0
+    c.k[hot, :, :, 5] = -127
+    c.ks[hot] = 2.0
+    c.vs[hot] *= 2.0 ** 60
+    out = torch.empty(queries, 4, d, device="cuda")
+    attend_cache(dav2lib, c, q, [160], [0, queries], False, out, 0.125)
+    assert ref.outside(out, want, bound) <= 1
