@@ -288,8 +288,9 @@ __global__ void __launch_bounds__(kThreads) attention_rows_kernel(const RowsPara
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
             // 2^e brings the row's largest value into [2^14, 2^15); rows of zeros, and
-            // exponents that would leave f32's range, stay near 1
-            int e = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
+            // exponents that would leave f32's range, stay near 1. Beside an infinity all finite
+            // values stay finite
+            int e = most > 0.0f ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
             e = max(-120, min(120, e));
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
             back = __uint_as_float((uint32_t)(127 - e) << 23);

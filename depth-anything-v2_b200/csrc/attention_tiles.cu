@@ -440,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const float2 v = unpack2(y[i], p.q_bf16);
                     most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
                 }
-                int ex = most > 0.0f && most < INFINITY ? 141 - (int)(__float_as_uint(most) >> 23) : 0;
+                int ex = most > 0.0f ? 141 - (int)(__float_as_uint(most) >> 23) : 0;  // an infinity: all finite ones stay so
                 ex = max(-120, min(120, ex));
                 const float up = __uint_as_float((uint32_t)(127 + ex) << 23);
                 c *= __uint_as_float((uint32_t)(127 - ex) << 23);

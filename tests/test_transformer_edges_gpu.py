@@ -90,3 +90,27 @@ def test_cache_attention_large_values_without_weight(cuda, dav2lib, queries, d, 
     out = torch.empty(queries, 4, d, device="cuda")
     attend_cache(dav2lib, c, q, [160], [0, queries], False, out, 0.125)
     assert ref.outside(out, want, bound) <= 1
+
+
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cache_attention_infinite_queries(cuda, dav2lib, queries, d):
+    """A query with -inf beside values above f16's range: keys that it scores -inf are left out (zeros if there is no
+    other), one of inf makes the row NaN."""
+    g = gen(35)
+    c = Cache(g, [150], 2, d, 32)
+    c.k[..., 5], c.k[..., 6] = 1, 1
+    q = randn(g, queries, 2, d, dtype=torch.bfloat16)
+    want, bound = ref.cache_attention(q, c.k, c.ks, c.v, c.vs, c.table, [150], [0, queries], 0.125, False, 0)
+    hurt = q.clone()
+    hurt[0, 1, 5], hurt[0, 1, 6] = -math.inf, 1e30
+    keep = torch.ones(queries, 2, d, dtype=torch.bool, device="cuda")
+    keep[0, 1] = False
+    out = torch.empty(queries, 2, d, device="cuda")
+    attend_cache(dav2lib, c, hurt, [150], [0, queries], False, out, 0.125)
+    assert (out[0, 1] == 0).all()
+    assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
+    hurt[0, 1, 5], hurt[0, 1, 6] = math.inf, -1e30
+    attend_cache(dav2lib, c, hurt, [150], [0, queries], False, out, 0.125)
+    assert out[0, 1].isnan().all()
+    assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
