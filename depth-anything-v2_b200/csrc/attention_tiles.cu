@@ -182,11 +182,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // 2^x of two values without the exponential unit, which the softmax would otherwise be
 // bound by (a quarter of the rate of a multiply-add): x = n + f with |f| <= 1/2, a
 // polynomial of degree 4 for 2^f (minimax in the relative error, 2.7e-6 as evaluated),
-// and n added to the exponent. x <= 127; below -126 the result is 2^-126, not 0, which a bf16 P
-// keeps: beside other values of V it counts where a value is above 2^100 times theirs.
+// and n added to the exponent. x <= 127; below -126 the result falls to 0 at -127 (the exponent is
+// then 0, and what is left of the polynomial a subnormal), about as a flush of subnormals would
+// have it. The lowest x is not -127 itself: the polynomial is below 1 at 0, and 1 less would be a
+// NaN's bits. 2^0.003 - 1 = 0.0021 leaves 0.0021 * 2^-126, which a 16-bit P rounds to 0.
 __device__ __forceinline__ void exp2_pair(float& x, float& y) {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it leaves rint(x) in the low bits
-    x = fmaxf(x, -126.0f), y = fmaxf(y, -126.0f);
+    x = fmaxf(x, -126.997f), y = fmaxf(y, -126.997f);
     float rx, ry, fx, fy, px, py;
     f2_add(rx, ry, x, y, kMagic, kMagic);
     f2_add(fx, fy, rx, ry, -kMagic, -kMagic);
@@ -605,7 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             looked = true;
             if (!warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
-            // a row that sees nothing: its P is 0 or, emulated, 2^-126. NaN, which raises no maximum, stays
+            // a row that sees nothing: its P is 0, but emulated ones leave 2^-135 in the sum. NaN, which raises
+            // no maximum, stays
             if (m == kLowest && l == l) l = 0.0f;
             if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
             constexpr float unit_v = kS8 ? 1.0f / 128.0f : 1.0f;

@@ -114,3 +114,22 @@ def test_cache_attention_infinite_queries(cuda, dav2lib, queries, d):
     attend_cache(dav2lib, c, hurt, [150], [0, queries], False, out, 0.125)
     assert out[0, 1].isnan().all()
     assert ref.outside(out[keep], want[keep], bound[keep]) <= 1
+
+
+@pytest.mark.parametrize("low", [-math.inf, -1e4])
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_cross_attention_keys_without_weight(cuda, dav2lib, queries, d, low):
+    """Keys whose score is -inf, or 1250 and more below the others, weigh nothing, however large their values: as
+    without them."""
+    g = gen(31)
+    q, k, v = (randn(g, 1, n, 2, d, dtype=torch.bfloat16) for n in (queries, 150, 150))
+    q[..., 5], k[..., 5] = 1.0, 0.0
+    gone = list(range(0, 150, 7))
+    k[:, gone, :, 5], v[:, gone] = low, 3e38
+    out = torch.empty(1, queries, 2, d, device="cuda")
+    cross(dav2lib, q, k, v, None, 0.125, out)
+    done(dav2lib)
+    rest = [i for i in range(150) if i not in gone]
+    want, bound = ref.cross_attention(q, k[:, rest], v[:, rest], [len(rest)], 0.125, 1, 0)
+    assert ref.outside(out, want, bound) <= 1
