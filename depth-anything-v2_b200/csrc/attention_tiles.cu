@@ -424,8 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 continue;
             }
             if (t >= w.tiles) continue;
-            // a negative scale is in the first product's sign; above 0, so that the -inf of a masked key stays
-            float c = fmaxf(fabsf(p.scale_log2), 1e-35f);
+            // a negative scale is in the first product's sign; 16-bit rows multiply by 0 where the mask is, whose
+            // -inf would not outlast it, and then by 1
+            const float once = kS8 || p.scale_log2 != 0.0f ? 1.0f : 0.0f;
+            float c = once != 0.0f ? fabsf(p.scale_log2) : 1.0f;
             if constexpr (kS8) {
                 // this row of Q, brought into f16's range by a power of two. The last unit's
                 // products are done: this warp has waited for its output.
@@ -462,7 +464,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 : p.splits > 1 ? part_at(p, w.where, w.kv_head, row, w.split)
                                                : row_at(p, w.where, w.kv_head, row, p.out_batch, p.out_stride);
             const uint32_t reach = reach_of(p, w.where, w.len, row);
-            const uint32_t low = __reduce_min_sync(0xffffffffu, live ? reach : 0xFFFFFFFFu);
+            // the first key that a row of the warp does not see; all keys go through the mask where `once` is 0
+            const uint32_t low = once == 0.0f ? 0u : __reduce_min_sync(0xffffffffu, live ? reach : 0xFFFFFFFFu);
             // codes: lane i has the K scale (i < 8), lane 8 + i the V scale, of the block's keys
             // 16i .. 16i + 15; fetched a block ahead. -1: no such page
             auto scale_of = [&](uint32_t j) -> float {
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (key0 + kKeys > low) {
 #pragma unroll
                     for (int i = 0; i < 128; ++i)
-                        if (key0 + i >= reach) s[i] = -INFINITY;
+                        s[i] = key0 + i >= reach ? -INFINITY : kS8 ? s[i] : s[i] * once;
                 }
                 // four chains: a tree's partial maxima beside 128 scores would not fit the registers
                 float a[4] = {s[0], s[1], s[2], s[3]};

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import transformer_ref as ref
-from test_transformer_ops_gpu import TYPES, Cache, attend_cache, cross, done, gen, randn
+from test_transformer_ops_gpu import TYPES, Cache, attend_cache, cross, done, gen, ints, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,33 @@ def test_cross_attention_keys_without_weight(cuda, dav2lib, queries, d, low):
     rest = [i for i in range(150) if i not in gone]
     want, bound = ref.cross_attention(q, k[:, rest], v[:, rest], [len(rest)], 0.125, 1, 0)
     assert ref.outside(out, want, bound) <= 1
+
+
+@pytest.mark.parametrize("queries", [1, 140])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_scale_zero_of_large_products(cuda, dav2lib, queries, d):
+    """scale 0 weighs all keys alike, however large q . k is, as long as it is finite."""
+    g = gen(34)
+    q, k, v = (randn(g, 1, n, 2, d, dtype=torch.bfloat16) for n in (queries, 150, 150))
+    q, k = q * 2.0 ** 60, k * 2.0 ** 60
+    out = torch.empty(1, queries, 2, d, device="cuda")
+    want, bound = ref.cross_attention(q * 0, k * 0, v, [150], 0.0, 1, 0)
+    for scale in (0.0, -0.0, 1e-44):
+        cross(dav2lib, q, k, v, None, scale, out)
+        done(dav2lib)
+        assert ref.outside(out, want, bound) <= 1
+    for low in (math.inf, -math.inf):  # 0 times an infinite product is NaN
+        hurt = k.clone()
+        hurt[0, 7, 1, 5] = low
+        cross(dav2lib, q, hurt, v, None, 0.0, out)
+        done(dav2lib)
+        assert out[:, :, 1].isnan().all() and ref.outside(out[:, :, 0], want[:, :, 0], bound[:, :, 0]) <= 1
+        cross(dav2lib, q, hurt, v, ints([7]), 0.0, out)
+        done(dav2lib)
+        short, within = ref.cross_attention(q * 0, k * 0, v, [7], 0.0, 1, 0)
+        assert ref.outside(out, short, within) <= 1
+    c = Cache(g, [150], 2, d, 16)
+    want, bound = ref.cache_attention(q[0] * 0, c.k, c.ks, c.v, c.vs, c.table, [150], [0, queries], 0.0, False, 0)
+    c.ks *= 2.0 ** 50
+    attend_cache(dav2lib, c, q[0], [150], [0, queries], False, out[0], 0.0)
+    assert ref.outside(out[0], want, bound) <= 1
