@@ -181,7 +181,9 @@ extern "C" DAV2CUDA_API int dav2cuda_cross_attention_16(
                  "cross attention: a token stride is below the row of its heads");
     DAV2_REQUIRE(keys <= 1 || (k_stride >= kv_row && v_stride >= kv_row),
                  "cross attention: a token stride is below the row of its heads");
-    DAV2_REQUIRE(batch == 1 || output_batch_stride >= (queries - 1) * output_stride + row,
+    // batch after batch, or (tokens first) the batches of a token one after another
+    DAV2_REQUIRE(batch == 1 || output_batch_stride >= (queries - 1) * output_stride + row ||
+                     (output_batch_stride >= row && output_stride >= (batch - 1) * output_batch_stride + row),
                  "cross attention: output batches overlap");
     DAV2_REQUIRE(!any_null(output, q) && (keys == 0 || !any_null(k, v)), "cross attention: null buffer");
     DAV2_REQUIRE(aligned16(output) && aligned16(q) && aligned16(k) && aligned16(v) &&

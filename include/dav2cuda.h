@@ -515,7 +515,8 @@ DAV2CUDA_API int dav2cuda_attention_cache_s8(void* output, const void* q, const 
  * into the result, whatever they hold; a batch entry without keys, or a row with
  * nothing but scores of -inf, gives zeros, a row with a score of inf or NaN NaN.
  * head_dim a multiple of 8 up to 128; 16-byte aligned rows; batch and token
- * strides as given. Query head h reads key head h / (q_heads / kv_heads). Output
+ * strides as given (0 for shared q, k or v; the output batch after batch or, with
+ * the token stride the larger, the batches of a token side by side). Query head h reads key head h / (q_heads / kv_heads). Output
  * f32 or of the operands' type. f32 accumulation, softmax weights rounded to the
  * operands' type. workspace_size answers for the same numbers. */
 DAV2CUDA_API uint64_t dav2cuda_cross_attention_16_workspace_size(uint32_t batch, uint32_t queries,

@@ -163,3 +163,19 @@ def test_attention_scale_zero_of_large_products(cuda, dav2lib, queries, d):
     c.ks *= 2.0 ** 50
     attend_cache(dav2lib, c, q[0], [150], [0, queries], False, out[0], 0.0)
     assert ref.outside(out[0], want, bound) <= 1
+
+
+@pytest.mark.parametrize("p,po", [(1, 0), (2, 2)])
+@pytest.mark.parametrize("batch,queries,keys,hq,hkv,d", [
+    (3, 1, 70, 4, 2, 64), (2, 5, 130, 4, 4, 128), (3, 140, 200, 4, 2, 64), (2, 300, 1000, 8, 2, 128), (3, 70, 90, 6, 2, 72)])
+def test_cross_attention_sequence_first(cuda, dav2lib, batch, queries, keys, hq, hkv, d, p, po):
+    """q, k, v and the output as [tokens][batch][heads][dim]: batch strides below the token strides."""
+    g = gen(36)
+    q, k, v = (randn(g, n, batch, h, d, dtype=TYPES[p]).transpose(0, 1) for n, h in ((queries, hq), (keys, hkv), (keys, hkv)))
+    held = torch.full((queries + 1, batch, hq, d), 5.0, dtype=TYPES[po], device="cuda")
+    out, lengths = held[:queries].transpose(0, 1), [keys - 7 * b for b in range(batch)]
+    cross(dav2lib, q, k, v, ints(lengths), 0.125, out)
+    done(dav2lib)
+    want, bound = ref.cross_attention(q, k, v, lengths, 0.125, p, po)
+    assert ref.outside(out, want, bound) <= 1
+    assert (held[queries:] == 5.0).all()

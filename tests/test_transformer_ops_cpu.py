@@ -160,3 +160,11 @@ def test_reference_append_matches_the_int8_rows_rule():
     packed, scale = oracle.quantize_rows_s8(x.numpy().reshape(1, -1), 1, 512)
     assert np.array_equal(codes.numpy().reshape(-1), np.asarray(packed).view(np.int8).reshape(-1))
     assert scales[0, 0] == np.asarray(scale).reshape(-1)[0]
+
+
+@pytest.mark.parametrize("change", [dict(ob=512, os=1016), dict(ob=504, os=4096), dict(ob=1528, os=512),
+                                    dict(batch=3, ob=512, os=1528)])
+def test_cross_attention_outputs_that_overlap(dav2lib, change):
+    """Rows of 512 values: neither a batch after the other nor the batches of a token side by side."""
+    assert dav2lib.dav2cuda_cross_attention_16(*cross_args(**change)) == 1
+    assert b"overlap" in dav2lib.dav2cuda_last_error()
