@@ -466,7 +466,8 @@ DAV2CUDA_API int dav2cuda_qk_norm_rope(void* q_output, void* k_output, const voi
  * holds. scale = max(absmax / 127, 1e-8) and code = rint(clamp(x / scale)) over
  * each page and head, as dav2cuda_quantize_rows_s8 has them for rows; a page that
  * holds tokens keeps its scale unless the new rows need a larger one, and its
- * codes then become rint(code * (old scale / new scale)). Infinities take the
+ * codes then become rint(code * (old scale / new scale)), which adds up to half a
+ * step of the new scale to their error each time. Infinities take the
  * codes +-127 and NaN the code 0; neither enters a scale. Places behind the last
  * token stay as they were. page_tokens 16, 32, 64 or 128, head_dim a multiple of
  * 16 up to 128. A page that receives rows may belong to one sequence only;

@@ -168,3 +168,29 @@ def test_cross_attention_outputs_that_overlap(dav2lib, change):
     """Rows of 512 values: neither a batch after the other nor the batches of a token side by side."""
     assert dav2lib.dav2cuda_cross_attention_16(*cross_args(**change)) == 1
     assert b"overlap" in dav2lib.dav2cuda_last_error()
+
+
+@pytest.mark.parametrize("grow", [1.0, 1.1])
+def test_reference_append_token_by_token(grow):
+    """A page filled by several calls: its scale is that of one call, its codes need not be. A value is off by half a
+    step of the scale that it was stored with and of each larger one since (and f32's roundings: a code times the
+    ratio, 127 at most, and the ratio itself, 2^-23 * 127 of a step each time)."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(64, 1, 64, generator=g) * grow ** torch.arange(64.0)[:, None, None]
+    codes, scales = torch.zeros(1, 1, 64, 64, dtype=torch.int8), torch.zeros(1, 1)
+    off = torch.zeros(64, dtype=torch.float64)
+    growths = 0
+    for t in range(64):
+        before = float(scales)
+        codes, scales = ref.append(codes, scales, x[t: t + 1], [[0]], [t], [0, 1])
+        now = float(scales)
+        step = 0.5 + 127 * 2.0 ** -23
+        off[t] = now * step
+        if t and now > before:
+            off[:t] += now * step
+            growths += 1
+    error = (codes[0, 0].double() * float(scales) - x[:, 0].double()).abs().amax(-1)
+    assert growths >= 2 and (error <= off).all()
+    once, scale = ref.append(torch.zeros_like(codes), torch.zeros(1, 1), x, [[0]], [0], [0, 64])
+    assert torch.equal(scale, scales) and not torch.equal(once, codes)
+    assert ((once[0, 0].double() * float(scale) - x[:, 0].double()).abs() <= float(scale) * step).all()
