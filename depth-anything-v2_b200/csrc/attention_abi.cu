@@ -50,6 +50,9 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_lengt
                                   (s > 1 ? 3 + s * part / 5000000 : 0);
             if (cost < best) best = cost, n.splits = (uint32_t)s;
         }
+        // warps that are done with a unit wait for the next one, and a wait ends with an error after 4 s
+        // (kWaitTimeoutNs): no unit is longer than 2^19 key blocks, under 2 s of 2 to 3.4 us each
+        n.splits = std::max(n.splits, (uint32_t)((blocks + (1u << 19) - 1) >> 19));
         return n;
     }
     // The rows kernel. What fits the device at once is filled by one wave of equal

@@ -194,3 +194,16 @@ def test_reference_append_token_by_token(grow):
     once, scale = ref.append(torch.zeros_like(codes), torch.zeros(1, 1), x, [[0]], [0], [0, 64])
     assert torch.equal(scale, scales) and not torch.equal(once, codes)
     assert ((once[0, 0].double() * float(scale) - x[:, 0].double()).abs() <= float(scale) * step).all()
+
+
+def test_workspace_of_the_longest_keys(dav2lib):
+    """Keys whose pass would outlast the kernels' bounded waits are split, also where there are rows for all SMs: no
+    part is longer than 2^26 keys."""
+    g, f = dav2lib.dav2cuda_cross_attention_16_workspace_size, dav2lib.dav2cuda_attention_cache_s8_workspace_size
+    rows = 148 * 256 * 4
+    for keys in (1 << 20, 1 << 26):
+        assert g(1, rows, keys, 1, 1, 64) == 0 and f(1, rows, keys, 1, 1, 128) == 0
+    for keys in ((1 << 26) + 1, 190_000_000, 0x7FFFFF00):
+        parts = -(-keys // (1 << 26))
+        assert g(1, rows, keys, 1, 1, 64) >= rows * parts * (64 * 4 + 8)
+        assert f(1, rows, keys, 1, 1, 128) >= rows * parts * (128 * 4 + 8)
