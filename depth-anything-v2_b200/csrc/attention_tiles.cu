@@ -34,7 +34,7 @@
 // that P's range is that of what the row's keys contribute (attention_rows.cuh).
 //
 // Bound by the softmax: for 128 keys an SM's four exponential units need 1.1 us at D = 64 and
-// 128 alike (0.8 with the polynomials), the products 0.65 and 1.1 us, and each tile's chain from
+// 128 alike, the products 0.65 and 1.1 us, and each tile's chain from
 // its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
 // other's alone.
 // Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 129 us (477 TFLOP/s); 4 x 1370 x 5477, 16
@@ -85,13 +85,6 @@ template <int D>
 constexpr bool kTurns = D == 128;
 
 constexpr float kLowest = -3.402823466e38f;
-// Of eight pairs of exponentials, how many leave the exponential unit alone. Measured with
-// 0, 1, 2, 3 of 8: 8 x 1370 x 1370, 16 heads of 64, 157, 142, 143, 140 us; 4 x 1370 x 5477,
-// 16 heads of 128, 229, 222, 221, 244 us. Codes, whose softmax shares the issue slots with the
-// conversion, are slower with any: 149, 151, 153, 156 us (700 queries over 6 caches).
-template <bool kS8>
-constexpr int kEmulated = kS8 ? 0 : 2;
-
 template <int D, bool kS8>
 struct Layout {
     static constexpr uint32_t kOperand = D / 64 * kAtom;   // bytes of 128 rows
@@ -177,29 +170,6 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-
-// 2^x of two values without the exponential unit, which the softmax would otherwise be
-// bound by (a quarter of the rate of a multiply-add): x = n + f with |f| <= 1/2, a
-// polynomial of degree 4 for 2^f (minimax in the relative error, 2.7e-6 as evaluated),
-// and n added to the exponent. x <= 127; below -126 the result falls to 0 at -127 (the exponent is
-// then 0, and what is left of the polynomial a subnormal), about as a flush of subnormals would
-// have it. The lowest x is not -127 itself: the polynomial is below 1 at 0, and 1 less would be a
-// NaN's bits. 2^0.003 - 1 = 0.0021 leaves 0.0021 * 2^-126, which a 16-bit P rounds to 0.
-__device__ __forceinline__ void exp2_pair(float& x, float& y) {
-    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: adding it leaves rint(x) in the low bits
-    x = fmaxf(x, -126.997f), y = fmaxf(y, -126.997f);
-    float rx, ry, fx, fy, px, py;
-    f2_add(rx, ry, x, y, kMagic, kMagic);
-    f2_add(fx, fy, rx, ry, -kMagic, -kMagic);
-    f2_fma(fx, fy, fx, fy, -1.0f, -1.0f, x, y);
-    f2_fma(px, py, fx, fy, 0.009570102207362652f, 0.009570102207362652f, 0.05591785907745361f, 0.05591785907745361f);
-    f2_fma(px, py, px, py, fx, fy, 0.240247443318367f, 0.240247443318367f);
-    f2_fma(px, py, px, py, fx, fy, 0.6931217908859253f, 0.6931217908859253f);
-    f2_fma(px, py, px, py, fx, fy, 0.9999992847442627f, 0.9999992847442627f);
-    // the magic number's own bits are shifted out
-    x = __int_as_float(__float_as_int(px) + (__float_as_int(rx) << 23));
-    y = __int_as_float(__float_as_int(py) + (__float_as_int(ry) << 23));
 }
 
 // A block's next unit, by taking over the place of a block that has not started:
@@ -574,8 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         float x = s[64 * h + 2 * i], y = s[64 * h + 2 * i + 1];
                         if constexpr (kS8) f2_add(x, y, x, y, off, off);
                         else f2_fma(x, y, x, y, c, c, off, off);
-                        if (i % 8 < kEmulated<kS8>) exp2_pair(x, y);
-                        else x = ex2_approx(x), y = ex2_approx(y);
+                        x = ex2_approx(x), y = ex2_approx(y);
                         if constexpr (kS8) {
                             constexpr int kPairs = 8;
                             const int e = 2 * (i & 1);
@@ -598,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (!ok) break;
                 l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-                if (top != top) l = top;  // a score is NaN: emulated exponentials would lose it
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -610,10 +578,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             looked = true;
             if (!warp_wait(&o_full[t], outs++)) break;
             tc_fence_after();
-            // a row that sees nothing: its P is 0, but emulated ones leave 2^-135 in the sum. NaN, which raises
-            // no maximum, stays
-            if (m == kLowest && l == l) l = 0.0f;
-            if (m == INFINITY) l = NAN;  // inf - inf, which they would lose too
             constexpr float unit_v = kS8 ? 1.0f / 128.0f : 1.0f;
             const float back = kShift != 0.0f ? 1.0f / 128.0f : 1.0f;
             const float f = l != 0.0f ? (p.splits == 1 ? unit_v / l : unit_v * back) : 0.0f;
