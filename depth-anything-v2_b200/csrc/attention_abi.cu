@@ -20,8 +20,9 @@ struct Plan {
     uint64_t slots;      // row blocks over all sequences
 };
 
-// Rows that share a key head decide the kernel. Keys are split where the row blocks
-// alone would leave SMs idle, down to 128 keys (tiles kernel: 256) to a block.
+// The rows that share a key head, of a sequence on average, decide the kernel for the whole
+// call: the host does not know the sequences' own. Keys are split where the row blocks
+// alone would leave SMs idle, down to 128 keys (tiles kernel: 512) to a block.
 Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_length, uint32_t group,
                uint32_t kv_heads, uint32_t head_dim) {
     const bool ragged = s8;  // query_begin gives the rows of a sequence
@@ -30,8 +31,8 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_lengt
     const uint64_t rows = each * group;
     n.row_tiles = rows <= 8 ? 1 : 2;
     n.row_warps = rows <= 16 ? 1 : 2;
-    // 32 and 64 rows of 64 dims over 2000 keys, rows and tiles kernel: 12.4 and 15.0, 19.5 and
-    // 16.0 us; 64 rows of 128 dims over 4000 tokens in the cache: 55 and 42 us
+    // 16 sequences of 16 key heads, 32 and 64 rows of 64 dims over 2000 keys, rows and tiles kernel: 38.5 and
+    // 54.0, 74.3 and 54.0 us; 8 caches of about 4000 tokens, 8 key heads, 64 rows of 128 dims: 82 and 51 us
     if (rows > 32) n.row_warps = 0;
     const uint64_t tile = n.row_warps ? 8ull * n.row_tiles * n.row_warps : 256;
     n.slots = ragged ? queries * group / tile + sequences : sequences * ((rows + tile - 1) / tile);
@@ -57,7 +58,7 @@ Plan plan_rows(uint64_t sequences, uint64_t queries, bool s8, uint32_t max_lengt
     }
     // The rows kernel. What fits the device at once is filled by one wave of equal
     // splits; where lengths may differ and are long, about two waves even out the end
-    // (48 streams of up to 8192 keys: 1, 2, 3 splits 134, 118, 124 us). Up to eight
+    // (48 streams of up to 8192 keys: 1, 2, 3 splits 123, 110, 113 us). Up to eight
     // splits are a cluster and join there, without the workspace and a second launch.
     const uint64_t fit = (uint64_t)kSms * (s8 ? (head_dim <= 64 ? 6 : 3) : 2);
     const uint64_t most = std::max<uint64_t>(1, max_length / 128);

@@ -38,10 +38,10 @@
 //
 // Codes: the conversion shares the issue slots with the loads (of an SM's four
 // instructions a cycle 2.6 are issued, over half of them for integer work), so that the
-// memory is not quite full: 200003 keys, 32 heads of 128 on 8 key heads, in 72 us (5.7
-// TB/s; without the rings 94 us); 48 streams of 2000 to 8192 keys, one token each, 111 us
-// (4.6 TB/s: lengths and waves are uneven). 16-bit rows: 16 streams of up to 1370 keys, 16
-// heads of 64, 15 us (4.6 TB/s). 1370 keys of one stream, 7.8 us: launch, a chain of four
+// memory is not quite full: 200003 keys, 32 heads of 128 on 8 key heads, in 71.3 us (5.7
+// TB/s; without the rings 94 us); 48 streams of 2000 to 8192 keys, one token each, 110 us
+// (4.7 TB/s: lengths and waves are uneven). 16-bit rows: 16 streams of up to 1370 keys, 16
+// heads of 64, 15.1 us (4.6 TB/s). 1370 keys of one stream, 7.2 us: launch, a chain of four
 // dependent loads, and the join.
 #include <algorithm>
 

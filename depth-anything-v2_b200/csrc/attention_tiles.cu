@@ -33,14 +33,14 @@
 // e to them and multiplies P by f before it is rounded, and the sum takes P times 2^-e, so
 // that P's range is that of what the row's keys contribute (attention_rows.cuh).
 //
-// Bound by the softmax: for 128 keys an SM's four exponential units need 1.1 us at D = 64 and
-// 128 alike, the products 0.65 and 1.1 us, and each tile's chain from
-// its scores to its next ones (load, maximum, exponentials, store, products) is hidden by the
-// other's alone.
-// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 129 us (477 TFLOP/s); 4 x 1370 x 5477, 16
-// heads of 128 on 4 key heads, padded batch, 220 us (873 TFLOP/s). Codes: the chain of one
+// No unit of the SM is full (16-bit rows: issue slots 34 to 38%, exponential unit 52%, tensor
+// pipe 25% at D = 64, 52% at D = 128): the time is each tile's chain from its scores to its next
+// ones (load, maximum, exponentials, store, products), hidden by the other tile's alone. For
+// 128 keys the exponential units need 1.1 us at D = 64 and 128 alike, the products 0.65 and 1.1.
+// Measured, bf16: 8 x 1370 x 1370, 16 heads of 64, 128 us (481 TFLOP/s); 4 x 1370 x 5477, 16
+// heads of 128 on 4 key heads, padded batch, 212 us (906 TFLOP/s). Codes: the chain of one
 // issuer and the conversion on top; 700 queries over 6 caches of up to 6000 tokens, 32 heads
-// of 128 on 8 key heads, 134 us (298 TFLOP/s).
+// of 128 on 8 key heads, 134 us (297 TFLOP/s).
 // Every wait is bounded (kWaitTimeoutNs); a timeout sets the device error word.
 #include <cudaTypedefs.h>
 

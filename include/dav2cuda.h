@@ -414,7 +414,9 @@ DAV2CUDA_API uint64_t dav2cuda_attention_head64_workspace_size(uint32_t batch, u
  * Device arrays of lengths, offsets and pages are read by the kernels; a value
  * out of range is never used as an address: the work that it belongs to is left
  * out (a length is clamped) and the device error word becomes 3; what the rows
- * concerned then hold is undefined.
+ * concerned then hold is undefined. Offsets (query_begin, token_begin) rise: one that
+ * is out of range, or below the one before it, may leave out rows of other sequences
+ * too.
  *
  * Outputs overlap no input, unless an entry says so. A workspace belongs to one
  * call at a time: calls that may run at once (on several streams, in several
@@ -435,8 +437,8 @@ DAV2CUDA_API int dav2cuda_rope_frequencies(float* host_frequencies, float* host_
 /* Norm of each head of q and k and rotation by position, in one pass.
  * q [tokens][q_heads][head_dim], k [tokens][k_heads][head_dim] (q_heads or
  * k_heads may be 0). norm: 0 none; 1 x * rsqrt(mean(x^2) + epsilon) * weight +
- * bias; 2 the same of x - mean(x); weight [head_dim] and bias [head_dim] f32,
- * each may be NULL (1 and 0). Then, with a = positions[token][axis] *
+ * bias; 2 the same of x - mean(x); sums in f32, also those of squares; weight
+ * [head_dim] and bias [head_dim] f32, each may be NULL (1 and 0). Then, with a = positions[token][axis] *
  * frequencies[pair] (positions NULL: the token's index; one axis), each pair
  * (u, v) of the first rotary_dim values becomes rotary_scale * (u cos a - v sin a,
  * v cos a + u sin a). layout: 0 pair i = values i and i + rotary_dim/2; 1 values
@@ -494,7 +496,8 @@ DAV2CUDA_API int dav2cuda_kv_cache_append_s8(int8_t* k_codes, float* k_scales, i
  * operands (codes exactly, q scaled by a power of two, softmax weights times the V
  * scale rounded to f16, relative to the row's largest: pages that a row does not see,
  * or gives no weight, cost it nothing) and f32 accumulation. workspace_size answers for
- * the same numbers. */
+ * the same numbers. One kernel, chosen by the mean number of queries, serves a call:
+ * prompts and single tokens are faster in calls of their own. */
 DAV2CUDA_API uint64_t dav2cuda_attention_cache_s8_workspace_size(uint32_t sequences, uint32_t queries,
                                                                  uint32_t max_length, uint32_t q_heads,
                                                                  uint32_t kv_heads, uint32_t head_dim);
@@ -519,7 +522,8 @@ DAV2CUDA_API int dav2cuda_attention_cache_s8(void* output, const void* q, const 
  * strides as given (0 for shared q, k or v; the output batch after batch or, with
  * the token stride the larger, the batches of a token side by side). Query head h reads key head h / (q_heads / kv_heads). Output
  * f32 or of the operands' type. f32 accumulation, softmax weights rounded to the
- * operands' type. workspace_size answers for the same numbers. */
+ * operands' type (bf16: those below 2^-126 of the row's largest are 0). workspace_size
+ * answers for the same numbers. */
 DAV2CUDA_API uint64_t dav2cuda_cross_attention_16_workspace_size(uint32_t batch, uint32_t queries,
                                                                  uint32_t keys, uint32_t q_heads,
                                                                  uint32_t kv_heads, uint32_t head_dim);
